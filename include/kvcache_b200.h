@@ -641,6 +641,86 @@ size_t kvb_decode_step_workspace_bytes(int B, int Hq, int Hkv, int history_count
 
 int kvb_decode_step(const kvb_decode_step_params* p, int device, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Serving requests of different lengths over paged K/V: plan, append, attend. No counterpart in
+ * the reference, whose batches share one length.
+ *
+ * Pools are bf16 or fp16 [num_pages,Hkv,page_tokens,D] (page_tokens a power of two; any strides
+ * that are multiples of 8 elements, D contiguous). Token t of request b is row t % page_tokens of
+ * page page_table[b, t / page_tokens]; its SLOT is page * page_tokens + row. Lengths, tables,
+ * slots and the free stack live on the device and are read there, so a step needs no host round
+ * trip and can be captured into a graph. What is wrong in device data (a page id or slot out of
+ * range, a table too short for a length) cannot be refused by the host: the access is skipped,
+ * zeros stand in for the row, and kvb_device_status reports KVB_BAD_ARG.
+ *
+ * kvb_page_plan: one step's bookkeeping. Request b keeps old = finished[b] ? 0 : kv_len[b] tokens
+ * and gets q_len[b] new ones. In request order, the pages of finished requests are pushed on the
+ * free stack (free_pages[0 .. *free_count), top last) and the pages the new tokens start are
+ * popped from it and entered in page_table.
+ *   finished        uint8 [B] or NULL (none); B <= 8192
+ *   cu_q            int32 [B+1] first new token of every request, and their number
+ *   kv_len_out      int32 [B] old + q_len; may be kv_len
+ *   free_count_out  int32 [1]; may be free_count
+ *   slot            int64 [capacity], position int32 [capacity] (old + index in the request),
+ *   request         int32 [capacity]; all three -1 behind the last new token
+ *   status          int32 [4]: pages lacking, tokens beyond capacity, requests that need more than
+ *                   W pages, 1 if the stack or a finished request's length cannot be (count outside
+ *                   [0, num_pages], more pages given back than there are). Unless all four are 0
+ *                   nothing changes: no page moves, cu_q is all 0, the slots are -1, lengths and
+ *                   count are copied.
+ * Negative lengths count as 0.
+ * ------------------------------------------------------------------------------------- */
+int kvb_page_plan(const int32_t* kv_len, const int32_t* q_len, const uint8_t* finished, int B,
+                  int32_t* page_table, int64_t page_table_stride, int W,
+                  int32_t* free_pages, int num_pages, const int32_t* free_count, int page_tokens, int capacity,
+                  int32_t* cu_q, int32_t* kv_len_out, int32_t* free_count_out,
+                  int64_t* slot, int32_t* position, int32_t* request, int32_t* status,
+                  int device, void* stream);
+
+/* Stores rows [N,Hkv,D] (16-bit elements of any type, D a multiple of 8, <= 1024; strides in
+ * elements, multiples of 8) at their slots; slot -1 is skipped. The same slot twice: one of the
+ * rows, which one is not defined. */
+int kvb_paged_append(const void* key, int64_t k_st, int64_t k_sh, const void* value, int64_t v_st, int64_t v_sh,
+                     const int64_t* slot, int N, int Hkv, int D,
+                     void* key_pool, int64_t kp_sp, int64_t kp_sh, int64_t kp_st,
+                     void* value_pool, int64_t vp_sp, int64_t vp_sh, int64_t vp_st,
+                     int num_pages, int page_tokens, int device, void* stream);
+
+/* Attention of the new tokens over everything their request holds, the new tokens included (their
+ * rows are in the pools already). Token i of request b stands at position p = kv_len - q_len + i
+ * and sees the keys j with
+ *     j < kv_len,   j <= p or j < prefix_len,   j > p - window (window > 0);
+ *     score = softcap * tanh(scaling * q.k / softcap) - slopes[head] * |p - j|
+ * (no cap when softcap is 0, no distance term without slopes). A token that sees no key gets a zero
+ * row and lse -inf. K and V at positions >= kv_len, or outside what any token of the call sees,
+ * are not read; values that some token of the request sees have to be finite.
+ * D is 64 or 128; any Hq that is a multiple of Hkv; scaling > 0, softcap >= 0, window >= 0. */
+typedef struct kvb_paged_attend_params {
+  const void* query;      int64_t q_st, q_sh;             /* [N,Hq,D]                  */
+  const void* key_pool;   int64_t k_sp, k_sh, k_st;       /* [num_pages,Hkv,page_tokens,D] */
+  const void* value_pool; int64_t v_sp, v_sh, v_st;
+  const int32_t* page_table; int64_t page_table_stride;   /* [B,W]                     */
+  const int32_t* kv_len;                                  /* [B] tokens held, new ones included */
+  const int32_t* cu_q;         /* [B+1] first row of every request in query and out; NULL: N == B, one token each.
+                                  Rows behind cu_q[B] are neither read nor written */
+  const int32_t* prefix_len;                              /* [B] or NULL               */
+  const float* slopes;                                    /* [Hq] or NULL              */
+  int elem_type;                                          /* 0 = bf16, 1 = fp16        */
+  int N, B, Hq, Hkv, D, W, num_pages, page_tokens;
+  int max_q;                   /* largest number of new tokens of a request, if known (0: unknown). Any value gives
+                                  the same result; it decides which kernel runs */
+  int window;
+  float scaling, softcap;
+  void* out;                                              /* [N,Hq,D] dense            */
+  float* lse;                                             /* fp32 [N,Hq] or NULL: natural log of the sum of exp(score) */
+  void* workspace; size_t workspace_bytes;
+} kvb_paged_attend_params;
+
+/* 0 for a shape that kvb_paged_attend refuses. */
+size_t kvb_paged_attend_workspace_bytes(int N, int B, int Hq, int Hkv, int W, int page_tokens, int D, int max_q);
+
+int kvb_paged_attend(const kvb_paged_attend_params* p, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

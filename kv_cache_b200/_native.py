@@ -55,6 +55,25 @@ class DecodeStepParams(C.Structure):
     ]
 
 
+class PagedAttendParams(C.Structure):
+    """Mirror of struct kvb_paged_attend_params."""
+
+    _fields_ = [
+        ("query", _p), ("q_st", _i64), ("q_sh", _i64),
+        ("key_pool", _p), ("k_sp", _i64), ("k_sh", _i64), ("k_st", _i64),
+        ("value_pool", _p), ("v_sp", _i64), ("v_sh", _i64), ("v_st", _i64),
+        ("page_table", _p), ("page_table_stride", _i64),
+        ("kv_len", _p), ("cu_q", _p), ("prefix_len", _p), ("slopes", _p),
+        ("elem_type", _i),
+        ("N", _i), ("B", _i), ("Hq", _i), ("Hkv", _i), ("D", _i), ("W", _i), ("num_pages", _i), ("page_tokens", _i),
+        ("max_q", _i),
+        ("window", _i),
+        ("scaling", _f), ("softcap", _f),
+        ("out", _p), ("lse", _p),
+        ("workspace", _p), ("workspace_bytes", _sz),
+    ]
+
+
 class ShardedStepParams(C.Structure):
     """Mirror of struct kvb_sharded_step_params."""
 
@@ -140,6 +159,11 @@ SIGNATURES = {
     "kvb_qabs_partial_scores": (_i, [_p, _p, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _p]),
     "kvb_qabs_candidate_full_scores": (_i, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _i, _i, _f, _p,
                                             _i, _i, _i, _i, _i, _i, _i, _p]),
+    "kvb_page_plan": (_i, [_p, _p, _p, _i, _p, _i64, _i, _p, _i, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _i, _p]),
+    "kvb_paged_append": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _i, _i, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                              _i, _i, _i, _p]),
+    "kvb_paged_attend_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "kvb_paged_attend": (_i, [C.POINTER(PagedAttendParams), _i, _p]),
     "kvb_decode_step_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "kvb_decode_step": (_i, [C.POINTER(DecodeStepParams), _i, _p]),
 }

@@ -14,6 +14,8 @@ capacity (``SparQMeanState.key_dim_major``, EVAL:2018-2042); this module gives K
   geometrically (one copy per doubling, not per token).
 * ``PreallocatedCache``  a ``transformers.Cache`` made of such layers; pass it as ``past_key_values``.
 
+``PagedKV`` (one length for the whole batch) and ``RequestPagedKV`` (every request its own) keep K/V in pages.
+
 The int4 side caches and fused-step workspaces stay in ``attention_patch.SparseDecodeState``; give it the same
 capacity (``state.capacity_hint``) and neither structure is ever re-allocated during a decode.
 """
@@ -22,6 +24,8 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+
+from . import ops
 
 try:                                                   # transformers is needed only for the Cache base classes
     from transformers.cache_utils import Cache, CacheLayerMixin
@@ -214,3 +218,52 @@ class PagedKV:
         k = self.key_pool[ids].permute(0, 2, 1, 3, 4).reshape(self.B, self.Hkv, pages * self.P, self.D)[:, :, :T]
         v = self.value_pool[ids].permute(0, 2, 1, 3, 4).reshape(self.B, self.Hkv, pages * self.P, self.D)[:, :, :T]
         return k.contiguous(), v.contiguous()
+
+
+class RequestPagedKV:
+    """K/V of up to ``max_requests`` requests of different lengths in pages, for all layers of a model: the layers have
+    their own pools ``[num_pages, Hkv, page_tokens, D]`` and share one page table, since a token has the same place in
+    all of them. All bookkeeping is device data that ``step`` updates with one kernel, so a serving step never waits for
+    the device and can be captured into a graph (``q_len`` and ``finished`` are then buffers the caller refills).
+
+        kv = RequestPagedKV(layers, max_requests, Hkv, D, page_tokens, num_pages, pages_per_request, device)
+        plan = kv.step(q_len, capacity)                   # q_len int32 [max_requests], 0 where a request is idle
+        for layer in range(layers):                       # rows of the step: plan.request, plan.position
+            kv.append(layer, key_rows, value_rows)        # [capacity, Hkv, D]
+            out = kv.attend(layer, query)                 # [capacity, Hq, D]
+    """
+
+    def __init__(self, num_layers: int, max_requests: int, kv_heads: int, head_dim: int, page_tokens: int, num_pages: int,
+                 pages_per_request: int, device, dtype: torch.dtype = torch.bfloat16):
+        if page_tokens < 1 or page_tokens & (page_tokens - 1):
+            raise ValueError("page_tokens must be a power of two")
+        self.page_tokens = int(page_tokens)
+        shape = (num_pages, kv_heads, page_tokens, head_dim)
+        self.key_pools = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.value_pools = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.page_table = torch.zeros((max_requests, pages_per_request), dtype=torch.int32, device=device)
+        self.kv_len = torch.zeros(max_requests, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.plan: Optional[ops.PagePlan] = None
+
+    def step(self, q_len: torch.Tensor, capacity: int, finished: Optional[torch.Tensor] = None) -> ops.PagePlan:
+        """Retires the ``finished`` requests and makes room for ``q_len[b]`` new tokens of every request (a finished
+        one starts over). ``capacity`` bounds their sum. The plan's ``status`` says whether there was room."""
+        self.plan = ops.page_plan(self.kv_len, q_len, self.page_table, self.free_pages, self.free_count, self.page_tokens,
+                                  capacity, finished=finished, in_place=True)
+        return self.plan
+
+    def _planned(self) -> ops.PagePlan:
+        if self.plan is None:
+            raise RuntimeError("call step() before append() and attend()")
+        return self.plan
+
+    def append(self, layer: int, key_rows: torch.Tensor, value_rows: torch.Tensor) -> None:
+        """Stores the step's rows ``[capacity, Hkv, D]``; those behind the last new token are ignored."""
+        ops.paged_append(key_rows, value_rows, self._planned().slot, self.key_pools[layer], self.value_pools[layer])
+
+    def attend(self, layer: int, query: torch.Tensor, **kwargs):
+        """``ops.paged_attend`` of the step's tokens ``[capacity, Hq, D]`` over their requests."""
+        return ops.paged_attend(query, self.key_pools[layer], self.value_pools[layer], self.page_table, self.kv_len,
+                                cu_q=self._planned().cu_q, **kwargs)

@@ -13,6 +13,8 @@
 #include "score_prefill_tc.cu"
 #include "score_prefill.cu"
 #include "qabs_fp32.cu"
+#include "page_plan.cu"
+#include "paged_attend.cu"
 
 extern "C" __attribute__((visibility("default"))) int kvb_version(void) { return 100; /* 0.1.0 */ }
 

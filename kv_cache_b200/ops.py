@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from ._native import DecodeStepParams, check
+from ._native import DecodeStepParams, PagedAttendParams, check
 
 HIST_BINS = 4096
 
@@ -735,6 +735,208 @@ def prefill_select_blocks(query: torch.Tensor, packed: torch.Tensor, scale: torc
     qcode, qscale = quantize_query_tokens(query, channel_idx)
     bs = score_prefill_blocks(qcode, qscale, packed, scale, key_count)
     return block_topk(bs, top_blocks), bs
+
+
+# ------------------------------------------------------------------------------------------
+# requests of different lengths over paged K/V: plan, append, attend
+# ------------------------------------------------------------------------------------------
+
+@dataclass
+class PagePlan:
+    """One serving step's bookkeeping (``page_plan``); everything is on the device."""
+    cu_q: torch.Tensor          # int32 [B+1] first new token of every request; cu_q[B] is their number
+    kv_len: torch.Tensor        # int32 [B] tokens held once the new ones are stored
+    free_count: torch.Tensor    # int32 [1] pages left on the free stack
+    slot: torch.Tensor          # int64 [capacity] page * page_tokens + row of every new token, -1 behind the last
+    position: torch.Tensor      # int32 [capacity] position in its request, -1 behind the last
+    request: torch.Tensor       # int32 [capacity] the request it belongs to, -1 behind the last
+    status: torch.Tensor        # int32 [4] all 0, or why nothing was planned (see page_plan)
+
+
+def _device_ints(name: str, t: torch.Tensor, n: Optional[int], device: torch.device, dtype=torch.int32) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a dense {str(dtype).split('.')[-1]} vector" + ("" if n is None else f" of {n}"))
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on {device}")
+    return t
+
+
+def _check_page_table(page_table: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1 \
+            or page_table.stride(1) != 1 or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
+        raise RuntimeError("page_table must be int32 [B, pages] with dense rows")
+    if page_table.device != device:
+        raise RuntimeError(f"page_table must be on {device}")
+    return page_table
+
+
+def _table_stride(page_table: torch.Tensor) -> int:
+    return max(page_table.stride(0), page_table.shape[1])
+
+
+def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+              free_count: torch.Tensor, page_tokens: int, capacity: int, *, finished: Optional[torch.Tensor] = None,
+              in_place: bool = False, out: Optional[PagePlan] = None) -> PagePlan:
+    """Gives the ``q_len[b]`` new tokens of every request a page and a row, on the device.
+
+    Request ``b`` holds ``kv_len[b]`` tokens in the pages ``page_table[b]`` (int32 ``[B, W]``), or starts over where
+    ``finished[b]`` (bool or uint8) is set: its pages then go back on the free stack ``free_pages[:free_count]`` before
+    new ones are taken, all in request order. ``page_table`` and ``free_pages`` are updated in place; the lengths and the
+    count are returned, and with ``in_place`` written to ``kv_len`` and ``free_count`` themselves (a captured step).
+    ``capacity``: size of the per-token outputs, at least the number of new tokens.
+
+    ``status`` of the result: pages lacking, tokens beyond ``capacity``, requests whose table row is too short, 1 if
+    the stack or a finished length cannot be. Unless all are 0 nothing is changed and no token has a slot."""
+    dev = kv_len.device
+    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if B < 1 or B > 8192:
+        raise RuntimeError("page_plan takes 1 to 8192 requests")
+    _device_ints("kv_len", kv_len, B, dev)
+    _device_ints("q_len", q_len, B, dev)
+    _check_page_table(page_table, B, dev)
+    _device_ints("free_pages", free_pages, None, dev)
+    _device_ints("free_count", free_count, 1, dev)
+    if page_tokens < 1 or page_tokens & (page_tokens - 1):
+        raise RuntimeError("page_tokens must be a power of two")
+    if capacity < 1 or free_pages.shape[0] < 1:
+        raise RuntimeError("capacity and the number of pages must be positive")
+    if finished is not None:
+        if finished.dtype not in (torch.bool, torch.uint8) or finished.shape != (B,) or not finished.is_contiguous() \
+                or finished.device != dev:
+            raise RuntimeError("finished must be a dense bool or uint8 vector, one element per request")
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=dev)
+        out = PagePlan(torch.empty(B + 1, **i32), kv_len if in_place else torch.empty(B, **i32),
+                       free_count if in_place else torch.empty(1, **i32),
+                       torch.empty(capacity, dtype=torch.int64, device=dev), torch.empty(capacity, **i32),
+                       torch.empty(capacity, **i32), torch.empty(4, **i32))
+    else:
+        if in_place and (out.kv_len is not kv_len or out.free_count is not free_count):
+            raise RuntimeError("in_place needs the plan's own kv_len and free_count")
+        for name, n in (("cu_q", B + 1), ("kv_len", B), ("free_count", 1), ("position", capacity), ("request", capacity),
+                        ("status", 4)):
+            _device_ints(name, getattr(out, name), n, dev)
+        _device_ints("slot", out.slot, capacity, dev, torch.int64)
+    check(_native.lib().kvb_page_plan(
+        kv_len.data_ptr(), q_len.data_ptr(), _ptr(finished), B, page_table.data_ptr(), _table_stride(page_table),
+        page_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), int(page_tokens), int(capacity),
+        out.cu_q.data_ptr(), out.kv_len.data_ptr(), out.free_count.data_ptr(), out.slot.data_ptr(), out.position.data_ptr(),
+        out.request.data_ptr(), out.status.data_ptr(), _dev(kv_len), _stream(dev)), "kvb_page_plan")
+    return out
+
+
+def _check_pools(key_pool: torch.Tensor, value_pool: torch.Tensor, device: torch.device) -> None:
+    if key_pool.dim() != 4 or value_pool.shape != key_pool.shape or value_pool.dtype != key_pool.dtype:
+        raise RuntimeError("key_pool and value_pool must be [num_pages,Hkv,page_tokens,D] of equal shape and type")
+    if key_pool.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("pools must be bf16 or fp16")
+    P = key_pool.shape[2]
+    if P < 1 or P & (P - 1):
+        raise RuntimeError("page_tokens must be a power of two")
+    for t in (key_pool, value_pool):
+        if t.device != device:
+            raise RuntimeError(f"pools must be on {device}")
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+            raise RuntimeError("pool rows must be contiguous and 16-byte aligned, strides multiples of 8 elements")
+
+
+def paged_append(key_rows: torch.Tensor, value_rows: torch.Tensor, slot: torch.Tensor, key_pool: torch.Tensor,
+                 value_pool: torch.Tensor) -> None:
+    """Stores new K and V rows ``[N,Hkv,D]`` (any token and head strides) at their ``slot`` (int64 ``[N]`` of
+    ``page_plan``) in the pools ``[num_pages,Hkv,page_tokens,D]``; rows whose slot is -1 are skipped. A slot that
+    appears twice receives one of its rows, which one is not defined."""
+    dev = key_pool.device
+    if key_rows.dim() != 3 or value_rows.shape != key_rows.shape:
+        raise RuntimeError("key_rows and value_rows must be [N,Hkv,D] of equal shape")
+    _check_pools(key_pool, value_pool, dev)
+    num_pages, Hkv, P, D = key_pool.shape
+    if key_rows.shape[1:] != (Hkv, D) or key_rows.dtype != key_pool.dtype or value_rows.dtype != key_pool.dtype:
+        raise RuntimeError("rows and pools must have the same heads, head size and type")
+    if key_rows.device != dev or value_rows.device != dev:
+        raise RuntimeError(f"rows must be on {dev}")
+    N = key_rows.shape[0]
+    _device_ints("slot", slot, N, dev, torch.int64)
+    if N == 0:
+        return
+    k, v = _rows_contiguous(key_rows), _rows_contiguous(value_rows)
+    check(_native.lib().kvb_paged_append(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slot.data_ptr(), N, Hkv, D,
+        key_pool.data_ptr(), *key_pool.stride()[:3], value_pool.data_ptr(), *value_pool.stride()[:3], num_pages, P,
+        _dev(key_pool), _stream(dev)), "kvb_paged_append")
+
+
+def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
+                 kv_len: torch.Tensor, *, cu_q: Optional[torch.Tensor] = None, max_q: int = 0,
+                 scaling: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                 window: int = 0, prefix_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                 return_lse: bool = False):
+    """Softmax attention of the new tokens of every request over all ``kv_len[b]`` tokens it holds in paged K/V, the
+    new ones included (``paged_append`` them first). ``query`` is ``[N,Hq,D]``, the requests' tokens one after the
+    other: rows ``cu_q[b] .. cu_q[b+1]`` (int32 ``[B+1]``) are the last tokens of request ``b``; without ``cu_q`` every
+    request has one. Rows behind ``cu_q[B]`` (a padded, captured batch) are left as they are. Returns ``[N,Hq,D]``.
+
+    Token at position ``p`` sees the keys ``j <= p``, and those below ``prefix_len[b]`` whatever ``p`` is, but none at or
+    below ``p - window`` when a window is given. Scores are ``scaling * q.k`` (default ``D ** -0.5``), capped to
+    ``softcap * tanh(. / softcap)`` when ``softcap > 0``, less ``slopes[head] * |p - j|`` when ``slopes`` (fp32 ``[Hq]``) are given.
+    ``return_lse`` also returns the fp32 ``[N,Hq]`` logarithm of each row's sum of exponentials. A row that sees no key
+    is zero, its logarithm -inf. ``max_q``: the largest number of new tokens of one request when the caller knows it;
+    it chooses the kernel and never the result. K and V rows that some token of their request sees must be finite."""
+    dev = query.device
+    if query.dim() != 3:
+        raise RuntimeError("query must be [N,Hq,D]")
+    _check_pools(key_pool, value_pool, dev)
+    N, Hq, D = query.shape
+    num_pages, Hkv, P, Dk = key_pool.shape
+    if query.dtype != key_pool.dtype:
+        raise RuntimeError("query and pools must have the same type")
+    if Dk != D or D not in (64, 128):
+        raise RuntimeError("head size must be 64 or 128, the same for query and pools")
+    if Hq < 1 or Hq % Hkv:
+        raise RuntimeError("the number of query heads must be a multiple of the number of KV heads")
+    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if B < 1 or B > 8192:
+        raise RuntimeError("paged_attend takes 1 to 8192 requests")
+    _device_ints("kv_len", kv_len, B, dev)
+    _check_page_table(page_table, B, dev)
+    if cu_q is not None:
+        _device_ints("cu_q", cu_q, B + 1, dev)
+    elif N != B:
+        raise RuntimeError("without cu_q every request has one token: query must have one row per request")
+    if prefix_len is not None:
+        _device_ints("prefix_len", prefix_len, B, dev)
+    if slopes is not None:
+        _device_ints("slopes", slopes, Hq, dev, torch.float32)
+    scaling = float(D) ** -0.5 if scaling is None else float(scaling)
+    if not 0.0 < scaling < 3.0e38 or not 0.0 <= softcap < 3.0e38 or window < 0 or max_q < 0:
+        raise RuntimeError("scaling must be positive and finite, softcap, window and max_q not negative")
+    query = _rows_contiguous(query)
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    elif out.shape != (N, Hq, D) or out.dtype != query.dtype or not out.is_contiguous() or out.device != dev \
+            or out.data_ptr() % 16:
+        raise RuntimeError("out must be a dense, 16-byte aligned tensor of the query's shape and type")
+    lse = torch.empty((N, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if N == 0:
+        return (out, lse) if return_lse else out
+    lib = _native.lib()
+    W = page_table.shape[1]
+    ws_bytes = lib.kvb_paged_attend_workspace_bytes(N, B, Hq, Hkv, W, P, D, int(max_q))
+    if ws_bytes == 0:
+        raise RuntimeError("kvb_paged_attend: unsupported shape")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    p = PagedAttendParams()
+    p.query, p.q_st, p.q_sh = query.data_ptr(), query.stride(0), query.stride(1)
+    p.key_pool, p.k_sp, p.k_sh, p.k_st = key_pool.data_ptr(), *key_pool.stride()[:3]
+    p.value_pool, p.v_sp, p.v_sh, p.v_st = value_pool.data_ptr(), *value_pool.stride()[:3]
+    p.page_table, p.page_table_stride = page_table.data_ptr(), _table_stride(page_table)
+    p.kv_len, p.cu_q, p.prefix_len, p.slopes = kv_len.data_ptr(), _ptr(cu_q), _ptr(prefix_len), _ptr(slopes)
+    p.elem_type = 0 if query.dtype == torch.bfloat16 else 1
+    p.N, p.B, p.Hq, p.Hkv, p.D, p.W, p.num_pages, p.page_tokens = N, B, Hq, Hkv, D, W, num_pages, P
+    p.max_q, p.window, p.scaling, p.softcap = int(max_q), int(window), scaling, float(softcap)
+    p.out, p.lse = out.data_ptr(), _ptr(lse)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), ws_bytes
+    check(lib.kvb_paged_attend(C.byref(p), _dev(query), _stream(dev)), "kvb_paged_attend")
+    return (out, lse) if return_lse else out
 
 
 # ------------------------------------------------------------------------------------------
