@@ -1,6 +1,6 @@
 // Attention of a ragged batch of new tokens over paged K/V: the kernel for few rows (decode steps, a handful of
 // drafted tokens) and the entry point. Scores, visible ranges, spans and pieces: paged_common.cuh.
-#include "paged_common.cuh"
+#include "paged_attend_tc.cu"
 
 namespace kvb {
 
@@ -291,9 +291,19 @@ static inline int64_t paged_tile_bound(int64_t N, int B, int Hkv, int G, int64_t
   const int64_t units = ((N * G + rows - 1) / rows + B) * Hkv;
   return units * ((keys + kt - 1) / kt + 1);
 }
-static inline int paged_rows_grid(int64_t N, int B, int Hkv, int G, int64_t keys) {
-  const int64_t t = paged_tile_bound(N, B, Hkv, G, keys, PR_ROWS, PR_KT);
-  return (int)(t < PR_MAX_GRID ? t : PR_MAX_GRID);
+// Few rows per request: the kernel bound by K and V bytes. More: the tensor-core kernel. Either takes any shape.
+static inline bool paged_few_rows(int N, int B, int G, int max_q) {
+  return (int64_t)(max_q > 0 ? max_q : N == B ? 1 : N) * G <= PR_ROWS;
+}
+struct PagedSizes { bool few; int grid, rows; };
+static inline PagedSizes paged_sizes(int N, int B, int Hkv, int G, int64_t keys, int max_q) {
+  PagedSizes s;
+  s.few = paged_few_rows(N, B, G, max_q);
+  s.rows = s.few ? PR_ROWS : PT_ROWS;
+  const int64_t most = s.few ? PR_MAX_GRID : PT_MAX_GRID;
+  const int64_t t = paged_tile_bound(N, B, Hkv, G, keys, s.rows, s.few ? PR_KT : PT_KT);
+  s.grid = (int)(t < most ? t : most);
+  return s;
 }
 static inline size_t paged_ws_bytes(int grid, int rows, int D) {
   return round_up((size_t)2 * grid * rows * D * 4, 256) + round_up((size_t)2 * grid * rows * 8, 256) + (size_t)2 * grid * 16;
@@ -317,8 +327,25 @@ static int launch_paged_rows(PagedParams& p, int device, cudaStream_t st) {
   return KVB_OK;
 }
 
+template <typename T, int D, bool MOD>
+static int launch_paged_chunk(PagedParams& p, int device, cudaStream_t st) {
+  static std::atomic<bool> done[KVB_MAX_DEVICES];
+  const int rc = ensure_dynamic_smem(paged_chunk_kernel<T, D, MOD>, done, device, PtCfg<D>::SMEM);
+  if (rc != KVB_OK) return rc;
+  static_assert(PA_MAX_B * 4 <= PtCfg<D>::OFF_BAR - PtCfg<D>::OFF_KV, "the scheduler's scratch is the ring");
+  KVB_CHECK_CUDA(launch_kernel(paged_chunk_kernel<T, D, MOD>, dim3(p.grid), dim3(PT_THREADS), PtCfg<D>::SMEM, st, p));
+  if (p.grid > 1) {
+    ChainLaunchScope chain;
+    chain.on();
+    KVB_CHECK_CUDA(launch_kernel(paged_merge_kernel<T, D, PT_ROWS, 4>, dim3(p.grid, PT_ROWS / (4 * PM_WARPS)),
+                                 dim3(PM_WARPS * 32), 0, st, p));
+  }
+  return KVB_OK;
+}
+
 template <typename T, int D>
-static int launch_paged(PagedParams& p, bool mod, int device, cudaStream_t st) {
+static int launch_paged(PagedParams& p, bool few, bool mod, int device, cudaStream_t st) {
+  if (!few) return mod ? launch_paged_chunk<T, D, true>(p, device, st) : launch_paged_chunk<T, D, false>(p, device, st);
   return mod ? launch_paged_rows<T, D, true>(p, device, st) : launch_paged_rows<T, D, false>(p, device, st);
 }
 
@@ -329,9 +356,9 @@ static int paged_shape(const kvb_paged_attend_params* p, int64_t& keys) {
   if (!page_tokens_ok(p->page_tokens)) return KVB_BAD_SHAPE;
   keys = (int64_t)p->W * p->page_tokens;
   if (keys > 0x40000000) return KVB_BAD_SHAPE;
-  // key tiles of one KV head of one request are counted in 32 bits
+  // rows, and key tiles of one KV head of one request, are counted in 32 bits
   const int64_t G = p->Hq / p->Hkv;
-  if (((int64_t)p->N * G / PR_ROWS + 1) * (keys / PR_KT + 2) > 0x7fffffff) return KVB_BAD_SHAPE;
+  if (p->N * G > 0x3fffffff || (p->N * G / PR_ROWS + 1) * (keys / PR_KT + 2) > 0x7fffffff) return KVB_BAD_SHAPE;
   return KVB_OK;
 }
 
@@ -344,7 +371,8 @@ extern "C" __attribute__((visibility("default"))) size_t kvb_paged_attend_worksp
   q.N = N; q.B = B; q.Hq = Hq; q.Hkv = Hkv; q.W = W; q.page_tokens = page_tokens; q.D = D; q.num_pages = 1;
   int64_t keys;
   if (paged_shape(&q, keys) != KVB_OK) return 0;
-  return paged_ws_bytes(paged_rows_grid(N, B, Hkv, Hq / Hkv, keys), PR_ROWS, D);
+  const PagedSizes s = paged_sizes(N, B, Hkv, Hq / Hkv, keys, max_q);
+  return paged_ws_bytes(s.grid, s.rows, D);
 }
 
 extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb_paged_attend_params* a, int device,
@@ -355,6 +383,7 @@ extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb
   int64_t keys;
   const int rc = paged_shape(a, keys);
   if (rc != KVB_OK) return rc;
+  if (a->max_q < 0) return KVB_BAD_ARG;
   if (a->page_table_stride < a->W || (a->cu_q == nullptr && a->N != a->B)) return KVB_BAD_SHAPE;
   if (a->elem_type != 0 && a->elem_type != 1) return KVB_BAD_ARG;
   if (!(a->scaling > 0.0f) || a->scaling > 3.0e38f || !(a->softcap >= 0.0f) || a->softcap > 3.0e38f || a->window < 0)
@@ -379,17 +408,18 @@ extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb
   p.scale_log2 = a->scaling * PA_LOG2E;
   if (a->softcap > 0.0f) { p.cap_in = a->scaling / a->softcap; p.cap_log2 = a->softcap * PA_LOG2E; }
   p.out = a->out; p.lse = a->lse;
-  p.grid = paged_rows_grid(a->N, a->B, a->Hkv, p.G, keys);
-  if (a->workspace_bytes < paged_ws_bytes(p.grid, PR_ROWS, a->D)) return KVB_WORKSPACE_TOO_SMALL;
+  const PagedSizes s = paged_sizes(a->N, a->B, a->Hkv, p.G, keys, a->max_q);
+  p.grid = s.grid;
+  if (a->workspace_bytes < paged_ws_bytes(s.grid, s.rows, a->D)) return KVB_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.ws_o = reinterpret_cast<float*>(ws);
-  ws += round_up((size_t)2 * p.grid * PR_ROWS * a->D * 4, 256);
+  ws += round_up((size_t)2 * s.grid * s.rows * a->D * 4, 256);
   p.ws_ml = reinterpret_cast<float2*>(ws);
-  ws += round_up((size_t)2 * p.grid * PR_ROWS * 8, 256);
+  ws += round_up((size_t)2 * s.grid * s.rows * 8, 256);
   p.ws_desc = reinterpret_cast<int4*>(ws);
   const bool mod = a->softcap > 0.0f || a->slopes != nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->elem_type == 0)
-    return a->D == 128 ? launch_paged<__nv_bfloat16, 128>(p, mod, device, st) : launch_paged<__nv_bfloat16, 64>(p, mod, device, st);
-  return a->D == 128 ? launch_paged<__half, 128>(p, mod, device, st) : launch_paged<__half, 64>(p, mod, device, st);
+    return a->D == 128 ? launch_paged<__nv_bfloat16, 128>(p, s.few, mod, device, st) : launch_paged<__nv_bfloat16, 64>(p, s.few, mod, device, st);
+  return a->D == 128 ? launch_paged<__half, 128>(p, s.few, mod, device, st) : launch_paged<__half, 64>(p, s.few, mod, device, st);
 }

@@ -1,0 +1,523 @@
+// Attention over paged K/V for chunks of new tokens, on the 5th-generation tensor cores. Scores, visible ranges, spans
+// and pieces: paged_common.cuh.
+#include "paged_common.cuh"
+#include "tcgen05.cuh"
+
+#include <type_traits>
+
+namespace kvb {
+
+constexpr int PT_ROWS = 256;                // rows of a unit: two accumulator tiles of 128
+constexpr int PT_MAX_GRID = 148;            // one block per SM
+constexpr int PT_KT = 128;                  // keys per tile
+constexpr int PT_THREADS = 512;             // warps 0-3, 4-7: softmax of row tile 0, 1; 8-11: loads; 12: MMA issue
+constexpr int PT_HALF = 128 * 128;          // bytes of 128 rows x 64 16-bit elements, 128-byte swizzle
+constexpr float PT_SHIFT = 7.0f;            // as in the kernel for few rows: weights reach 2^7, stale ones 2^15
+constexpr float PT_LAZY = 8.0f;
+
+template <int D>
+struct PtCfg {
+  static constexpr int NH = D / 64;                      // 64-element halves of a row
+  static constexpr int TILEB = NH * PT_HALF;             // one 128-row operand tile
+  static constexpr int ST = D == 128 ? 5 : 8;            // K/V ring stages
+  static constexpr int LAG = ST - 2 < 4 ? ST - 2 : 4;    // loads in flight behind the newest one
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_KV = 2 * TILEB;
+  static constexpr int OFF_BAR = OFF_KV + ST * TILEB;
+  static constexpr int Q_FULL = OFF_BAR, Q_EMPTY = Q_FULL + 8, FULL = Q_EMPTY + 8, EMPTY = FULL + 8 * ST;   // barriers
+  static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 16;
+  static constexpr int OFF_MISC = DONE + 8;                                                             // tmem base, dead
+  static constexpr int BYTES = OFF_MISC + 16;
+  static constexpr int SMEM = BYTES + 1024;              // the base is brought to a swizzle atom
+  static constexpr uint32_t TS = 0, TO = 256;            // tensor memory: scores at 128*w, outputs at 256 + D*w
+};
+
+__device__ __forceinline__ uint64_t pt_desc(uint32_t addr, uint32_t lbo) {
+  // 128-byte swizzle, 8-row groups 1024 bytes apart
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_mn_major) {
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t t, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
+      "%25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+      "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]),
+      "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Barriers by shared-memory address (one register instead of two).
+__device__ __forceinline__ void pt_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait that also gives up once another role of the block has (`dead`: a shared word).
+__device__ __forceinline__ bool pt_wait(uint32_t bar, uint32_t parity, uint32_t dead) {
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ok) : "r"(dead) : "memory");
+    if (ok) return false;
+  }
+  asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(dead), "r"(1u) : "memory");
+  atomicExch(&g_device_status, (int)KVB_TIMEOUT);
+  return false;
+}
+
+// The part of a unit that a block has: key tiles [n0, n1), and those that row tile w works on, [na, nb).
+struct PtPiece {
+  PagedUnit<PT_ROWS, PT_KT> u;
+  int n0, n1;
+  bool begins, ends;
+  __device__ __forceinline__ void set(const PagedParams& p, const PagedPlace& at, const PagedRequest& r, long long left) {
+    u.set(r, p.G, p.window, at.tile);
+    n0 = u.t0 + at.k;
+    n1 = n0 + (int)min((long long)(u.n - at.k), left);
+    begins = at.k == 0;
+    ends = n1 == u.t0 + u.n;
+  }
+  __device__ __forceinline__ void rows(const PagedParams& p, const PagedPlace& at, const PagedRequest& r, int w, int& na,
+                                       int& nb) const {
+    na = nb = n0;
+    const int f0 = at.tile * PT_ROWS + w * 128;
+    if (f0 >= r.q * p.G) return;
+    const int lo = paged_lo(r, p.window, f0 / p.G), hi = paged_hi(r, min(r.q - 1, (f0 + 127) / p.G));
+    if (hi <= lo) return;
+    const int a = max(n0, lo / PT_KT), b = min(n1, (hi + PT_KT - 1) / PT_KT);
+    if (a < b) { na = a; nb = b; }
+  }
+};
+
+// ---- loads: 4 warps, each 32 rows of every operand tile --------------------------------------------------
+template <typename T, int D>
+struct PtLoader {
+  using Cfg = PtCfg<D>;
+  static constexpr int CPR = D / 8, RPI = 32 / CPR;
+  const PagedParams& p;
+  uint32_t base;
+  int w, lane;
+  int item, sent;                                        // K/V tiles requested, and handed to the tensor core
+
+  __device__ __forceinline__ PtLoader(const PagedParams& p_, uint32_t base_, int w_, int lane_)
+      : p(p_), base(base_), w(w_), lane(lane_), item(0), sent(0) {}
+
+  __device__ __forceinline__ void signal(uint32_t bar) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) pt_arrive(bar);
+  }
+  __device__ __forceinline__ void flush() {
+    cp_async_wait<0>();
+    for (; sent < item; ++sent) signal(base + Cfg::FULL + 8 * (sent % Cfg::ST));
+  }
+  // page of this lane's row of key tile n, or -1 (row not seen by the unit, or a bad table entry)
+  __device__ __forceinline__ int page_of(const PtPiece& pc, const int32_t* table, int n) const {
+    const int t = n * PT_KT + 32 * w + lane;
+    if (n >= pc.n1 || t < pc.u.lo || t >= pc.u.hi) return -1;
+    const int page = table[t >> p.shift];
+    if (page < 0 || page >= p.num_pages) {
+      atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+      return -1;
+    }
+    return page;
+  }
+  __device__ __forceinline__ bool load_rows(const T* pool, int64_t sp, int64_t st, int n, int page) {
+    const int stage = item % Cfg::ST;
+    if (!pt_wait(base + Cfg::EMPTY + 8 * stage, ((item / Cfg::ST) & 1) ^ 1, base + Cfg::OFF_MISC + 4)) return false;
+    const uint32_t dst = base + Cfg::OFF_KV + stage * Cfg::TILEB;
+    const int c = lane % CPR, mask = (1 << p.shift) - 1;
+    const uint32_t col = dst + (c >> 3) * PT_HALF;
+#pragma unroll
+    for (int j = 0; j < 32 / RPI; ++j) {
+      const int row = lane / CPR + j * RPI, ra = 32 * w + row;
+      const int pg = __shfl_sync(0xffffffffu, page, row);
+      const bool ok = pg >= 0;
+      const int64_t at = ok ? (int64_t)pg * sp + (int64_t)((n * PT_KT + ra) & mask) * st + c * 8 : 0;
+      cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), pool + at, ok);
+    }
+    cp_async_commit();
+    ++item;
+    if (item - sent > Cfg::LAG) {
+      cp_async_wait<Cfg::LAG>();
+      signal(base + Cfg::FULL + 8 * (sent % Cfg::ST));
+      ++sent;
+    }
+    return true;
+  }
+  __device__ __forceinline__ void load_query(const PagedPlace& at, const PagedRequest& r) {
+    const int total = r.q * p.G;
+#pragma unroll
+    for (int tl = 0; tl < 2; ++tl) {
+      if (at.tile * PT_ROWS + tl * 128 >= total) break;
+      const int flat = at.tile * PT_ROWS + tl * 128 + 32 * w + lane;
+      int64_t off = -1;
+      if (flat < total) {
+        const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
+        off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
+      }
+      const int c = lane % CPR;
+      const uint32_t col = base + Cfg::OFF_Q + tl * Cfg::TILEB + (c >> 3) * PT_HALF;
+#pragma unroll 4
+      for (int j = 0; j < 32 / RPI; ++j) {
+        const int row = lane / CPR + j * RPI, ra = 32 * w + row;
+        const int64_t o = __shfl_sync(0xffffffffu, off, row);
+        const bool ok = o >= 0;
+        cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), reinterpret_cast<const T*>(p.q) + (ok ? o + c * 8 : 0), ok);
+      }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    signal(base + Cfg::Q_FULL);
+  }
+  __device__ __forceinline__ void run(PagedPlace at, PagedRequest r, long long left) {
+    uint32_t unit = 0;
+    while (true) {
+      PtPiece pc;
+      pc.set(p, at, r, left);
+      const int32_t* table = p.table + (int64_t)at.b * p.table_st;
+      const T* kp = reinterpret_cast<const T*>(p.key) + (int64_t)at.h * p.k_sh;
+      const T* vp = reinterpret_cast<const T*>(p.value) + (int64_t)at.h * p.v_sh;
+      int page = page_of(pc, table, pc.n0);
+      bool ok = true;
+      for (int n = pc.n0; n < pc.n1 && ok; ++n) {
+        const int next = page_of(pc, table, n + 1);
+        ok = load_rows(kp, p.k_sp, p.k_st, n, page) && load_rows(vp, p.v_sp, p.v_st, n, page);
+        if (ok && n == pc.n0) {
+          // the next unit's first keys are on their way before the last unit's query is given up
+          flush();
+          ok = pt_wait(base + Cfg::Q_EMPTY, (unit & 1) ^ 1, base + Cfg::OFF_MISC + 4);
+          if (ok) load_query(at, r);
+        }
+        page = next;
+      }
+      if (!ok) break;
+      ++unit;
+      left -= pc.n1 - pc.n0;
+      if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
+    }
+    flush();
+  }
+};
+
+// ---- MMA issue: one thread -------------------------------------------------------------------------------
+template <typename T, int D>
+__device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base, uint32_t tmem, PagedPlace at, PagedRequest r, long long left) {
+  using Cfg = PtCfg<D>;
+  const uint32_t full = base + Cfg::FULL, empty = base + Cfg::EMPTY, s_full = base + Cfg::S_FULL, p_full = base + Cfg::P_FULL;
+  const uint32_t dead = base + Cfg::OFF_MISC + 4;
+  constexpr uint32_t id_s = pt_idesc<T>(PT_KT, false), id_o = pt_idesc<T>(D, true);
+  int item = 0;
+  uint32_t unit = 0, p_use[2] = {0, 0};
+  bool ok = true;
+  auto ring = [&](int it) { return base + Cfg::OFF_KV + (it % Cfg::ST) * Cfg::TILEB; };
+  auto scores = [&](int w, uint32_t k) {
+    const uint32_t q = base + Cfg::OFF_Q + w * Cfg::TILEB;
+#pragma unroll
+    for (int h = 0; h < Cfg::NH; ++h)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        pt_mma_ss(tmem + Cfg::TS + 128 * w, pt_desc(q + h * PT_HALF + s * 32, 16), pt_desc(k + h * PT_HALF + s * 32, 16), id_s,
+                  h + s > 0 ? 1u : 0u);
+  };
+  while (ok) {
+    PtPiece pc;
+    pc.set(p, at, r, left);
+    int na[2], nb[2];
+    pc.rows(p, at, r, 0, na[0], nb[0]);
+    pc.rows(p, at, r, 1, na[1], nb[1]);
+    // first keys and the query
+    if (!pt_wait(full + 8 * (item % Cfg::ST), (item / Cfg::ST) & 1, dead) || !pt_wait(base + Cfg::Q_FULL, unit & 1, dead)) { ok = false; break; }
+    tc_fence_after();
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (na[w] == pc.n0 && nb[w] > na[w]) {
+        scores(w, ring(item));
+        pt_commit(s_full + 8 * w);
+      }
+    pt_commit(empty + 8 * (item % Cfg::ST));
+    for (int n = pc.n0; n < pc.n1; ++n) {
+      const int v = item + 1, k = item + 2;
+      const bool more = n + 1 < pc.n1;
+      if (!pt_wait(full + 8 * (v % Cfg::ST), (v / Cfg::ST) & 1, dead) || (more && !pt_wait(full + 8 * (k % Cfg::ST), (k / Cfg::ST) & 1, dead))) {
+        ok = false;
+        break;
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const bool pv = n >= na[w] && n < nb[w], sc = n + 1 >= na[w] && n + 1 < nb[w];
+        if (pv) {
+          if (!pt_wait(p_full + 8 * w, p_use[w] & 1, dead)) { ok = false; break; }
+          ++p_use[w];
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < PT_KT / 16; ++j)
+            pt_mma_ts(tmem + Cfg::TO + D * w, tmem + Cfg::TS + 128 * w + 8 * j, pt_desc(ring(v) + j * 2048, PT_HALF), id_o,
+                      (n > na[w] || j > 0) ? 1u : 0u);
+        }
+        if (sc) scores(w, ring(k));
+        if (pv || sc) pt_commit(s_full + 8 * w);
+      }
+      if (!ok) break;
+      pt_commit(empty + 8 * (v % Cfg::ST));
+      if (more) pt_commit(empty + 8 * (k % Cfg::ST));
+      item += 2;
+    }
+    if (!ok) break;
+    pt_commit(base + Cfg::Q_EMPTY);
+    ++unit;
+    left -= pc.n1 - pc.n0;
+    if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
+  }
+  pt_commit(base + Cfg::DONE);
+  pt_wait(base + Cfg::DONE, 0, dead);
+}
+
+// ---- softmax of one row tile: 4 warps, one row per thread ------------------------------------------------
+template <typename T, int D, bool MOD>
+__device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, uint32_t tmem, int w, int tid, PagedPlace at, PagedRequest r, long long left) {
+  using Cfg = PtCfg<D>;
+  const uint32_t s_full = base + Cfg::S_FULL + 8 * w, p_full = base + Cfg::P_FULL + 8 * w, dead = base + Cfg::OFF_MISC + 4;
+  const int warp = tid >> 5, lane = tid & 31;
+  const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+  const uint32_t ts = tmem + Cfg::TS + 128 * w + lanes, to = tmem + Cfg::TO + D * w + lanes;
+  uint32_t s_use = 0;
+  while (true) {
+    PtPiece pc;
+    pc.set(p, at, r, left);
+    int na, nb;
+    pc.rows(p, at, r, w, na, nb);
+    const int flat = at.tile * PT_ROWS + w * 128 + tid;
+    const bool live = flat < r.q * p.G;
+    const int token = live ? flat / p.G : 0, head = at.h * p.G + (live ? flat - token * p.G : 0);
+    const int pos = r.kv - r.q + token;
+    const int lo = live ? paged_lo(r, p.window, token) : 0, hi = live ? max(lo, paged_hi(r, token)) : 0;
+    const float slope = MOD && p.slopes && live ? p.slopes[head] * PA_LOG2E : 0.0f;
+    // keys that every row of the tile sees need no mask
+    const int f0 = at.tile * PT_ROWS + w * 128;
+    const int all_lo = paged_lo(r, p.window, min(r.q - 1, (f0 + 127) / p.G)), all_hi = paged_hi(r, f0 / p.G);
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int n = na; n < nb; ++n) {
+      if (!pt_wait(s_full, s_use & 1, dead)) { ok = false; break; }
+      ++s_use;
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) TcLd<32>::ld(ts + 32 * c, v[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) TcLd<32>::wait(v[c]);
+      const int t0 = n * PT_KT;
+      if constexpr (MOD) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[c][i] = __float_as_uint(paged_score(p, __uint_as_float(v[c][i]), slope, pos, t0 + 32 * c + i));
+      }
+      if (t0 < all_lo || t0 + PT_KT > all_hi) {
+        const uint32_t from = (uint32_t)(lo - t0), width = (uint32_t)(hi - lo);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if ((uint32_t)(32 * c + i) - from >= width) v[c][i] = 0xff800000u;
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+        for (int i = 1; i < 31; i += 2)
+          asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[c]) : "f"(__uint_as_float(v[c][i])), "f"(__uint_as_float(v[c][i + 1])));
+        mx[c] = fmaxf(mx[c], __uint_as_float(v[c][31]));
+      }
+      const float scale = MOD ? 1.0f : p.scale_log2;
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale - PT_SHIFT;
+      const bool move = top > m + PT_LAZY;
+      if (__any_sync(0xffffffffu, move)) {
+        const float mn = move ? top : m, a = move ? ex2(m - mn) : 1.0f;
+        m = mn;
+        l *= a;
+        if (n > na) {                                    // the product before this one is complete: it was issued before these scores
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            TcLd<32>::ld(to + 32 * c, o);
+            TcLd<32>::wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+            tc_st32(to + 32 * c, o);
+          }
+        }
+      }
+      const float ms = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int e = 64 * c + 2 * i;
+          const float x = ex2(fmaf(__uint_as_float(v[e >> 5][e & 31]), scale, -ms));
+          const float y = ex2(fmaf(__uint_as_float(v[e >> 5][(e & 31) + 1]), scale, -ms));
+          sum[2 * (i & 1)] += x;
+          sum[2 * (i & 1) + 1] += y;
+          pk[i] = Half2Of<T>::pack(x, y);
+        }
+        tc_st32(ts + 32 * c, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) pt_arrive(p_full);
+    }
+    if (!ok) return;
+    // ---- the unit, or this block's piece of it
+    const bool some = nb > na;
+    if (some) {
+      if (!pt_wait(s_full, s_use & 1, dead)) return;
+      ++s_use;
+      tc_fence_after();
+    }
+    const bool whole = pc.begins && pc.ends;
+    const int slot = 2 * blockIdx.x + (pc.begins ? 1 : 0);
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const int64_t row = (int64_t)(r.first + token) * p.Hq + head;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32];
+      if (some) {
+        TcLd<32>::ld(to + 32 * c, o);
+        TcLd<32>::wait(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      if (!live) continue;
+      if (whole) {
+        uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * D + 32 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = Half2Of<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+          out[i] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+      } else {
+        uint4* dst = reinterpret_cast<uint4*>(p.ws_o + ((int64_t)slot * PT_ROWS + w * 128 + tid) * D + 32 * c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      }
+    }
+    if (live) {
+      if (!whole) p.ws_ml[(int64_t)slot * PT_ROWS + w * 128 + tid] = make_float2(m, l);
+      else if (p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * PA_LN2;
+    }
+    if (!whole && w == 0 && tid == 0)
+      p.ws_desc[slot] = pc.begins ? make_int4(1, at.b, at.h, at.tile) : make_int4(1, pc.ends ? 1 : 0, 0, 0);
+    tc_fence_before();                                   // the next unit's product overwrites the output once its weights are signalled
+    left -= pc.n1 - pc.n0;
+    if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) return;
+  }
+}
+
+// A block walks its span unit by unit: 4 warps copy K and V tiles (and each unit's query rows) into shared memory in the
+// 128-byte-swizzled layout, one thread issues S_w = Q_w K^T and O_w += P_w V for two row tiles w of 128 rows, and four
+// warps per row tile, one row per thread, turn scores into weights: S_w is read from tensor memory, P_w goes back over
+// it as 16-bit operand of the second product, and O_w stays in tensor memory until the unit ends. While the softmax of
+// one row tile runs, the tensor core works on the other. The reference of a row moves only when a score passes it by
+// 2^8, so O_w is rescaled rarely, and then by the softmax warps, which know from the order of issue that the previous
+// product is complete. Rows of K and V outside what the unit sees are zero-filled, not read.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_chunk_kernel(PagedParams p) {
+  using Cfg = PtCfg<D>;
+  extern __shared__ uint8_t pt_raw[];
+  const uint32_t raw = smem_u32(pt_raw);
+  uint8_t* smem = pt_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t base = smem_u32(smem);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+
+  PagedPlace at;
+  long long left;
+  paged_span<PT_ROWS, PT_KT, PT_THREADS>(p, reinterpret_cast<int*>(smem + Cfg::OFF_KV), at, left, 2);
+  if (tid < 2) p.ws_desc[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
+  if (left <= 0) return;
+  if (warp == 0) {
+    tc_alloc(s_tmem, 512);
+    tc_relinquish();
+  }
+  if (tid == 32) {
+    s_tmem[1] = 0;
+    auto bar = [&](int off) { return reinterpret_cast<uint64_t*>(smem + off); };
+    mbar_init(bar(Cfg::Q_FULL), 4);
+    mbar_init(bar(Cfg::Q_EMPTY), 1);
+    for (int i = 0; i < Cfg::ST; ++i) {
+      mbar_init(bar(Cfg::FULL + 8 * i), 4);
+      mbar_init(bar(Cfg::EMPTY + 8 * i), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(bar(Cfg::S_FULL + 8 * w), 1);
+      mbar_init(bar(Cfg::P_FULL + 8 * w), 4);
+    }
+    mbar_init(bar(Cfg::DONE), 1);
+    fence_mbar_init();
+  }
+  const PagedRequest r = paged_request(p, at.b);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  // registers: 128 x 512 at launch = 192 x 256 + 64 x 256
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    pt_softmax<T, D, MOD>(p, base, tmem, warp >> 2, tid & 127, at, r, left);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp < 12) {
+      PtLoader<T, D> loader(p, base, warp - 8, lane);
+      loader.run(at, r, left);
+    } else if (warp == 12 && lane == 0) {
+      pt_issue<T, D>(p, base, tmem, at, r, left);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tc_dealloc(tmem, 512);
+}
+
+}  // namespace kvb
