@@ -172,14 +172,25 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
       const bool edge = t0 < all_lo || t0 + 16 > all_hi;
       float x[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int t = t0 + 8 * n + 2 * t4 + (e & 1), w = e >> 1;
-          float v = MOD ? paged_score(p, c[n][e], slope[w], pos[w], t) : c[n][e] * p.scale_log2;
-          if (edge && (t < lo[w] || t >= hi[w])) v = -INFINITY;
-          x[n][e] = v;
+        for (int w = 0; w < 2; ++w) {
+          if constexpr (MOD) {
+            x[n][2 * w] = c[n][2 * w];
+            x[n][2 * w + 1] = c[n][2 * w + 1];
+            paged_scores<2>(p, &x[n][2 * w], slope[w], t0 + 8 * n + 2 * t4 - pos[w]);
+          } else {
+            x[n][2 * w] = c[n][2 * w] * p.scale_log2;
+            x[n][2 * w + 1] = c[n][2 * w + 1] * p.scale_log2;
+          }
         }
+        if (edge)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = t0 + 8 * n + 2 * t4 + (e & 1), w = e >> 1;
+            if (t < lo[w] || t >= hi[w]) x[n][e] = -INFINITY;
+          }
+      }
       float mx[2];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[n][e] = exp2f(x[n][e] - ms[e >> 1]);
+          x[n][e] = ex2(x[n][e] - ms[e >> 1]);
           l[e >> 1] += x[n][e];
         }
       uint32_t pa[4];
@@ -327,13 +338,48 @@ static int launch_paged_rows(PagedParams& p, int device, cudaStream_t st) {
   return KVB_OK;
 }
 
+// The pool as a 4-D tensor (element of a row, row of a page, KV head, page) in boxes of 64 elements x min(page, 128)
+// rows, 128-byte swizzle: the layout the tensor core reads. False when the driver takes no such map (a stride of 0, or
+// beyond its range); rows are then copied one by one.
+template <typename T>
+static bool paged_tensor_map(CUtensorMap* map, const void* pool, int64_t sp, int64_t sh, int64_t st, int D, int P, int Hkv, int pages) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess) fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode || P < 8 || st < D || (Hkv > 1 && sh < D) || (pages > 1 && sp < D)) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)P, (cuuint64_t)Hkv, (cuuint64_t)pages};
+  // a dimension of one element has no stride of its own
+  const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)(Hkv > 1 ? sh : D) * 2, (cuuint64_t)(pages > 1 ? sp : D) * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)(P < PT_KT ? P : PT_KT), 1, 1}, step[4] = {1, 1, 1, 1};
+  return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, bool MOD>
 static int launch_paged_chunk(PagedParams& p, int device, cudaStream_t st) {
   static std::atomic<bool> done[KVB_MAX_DEVICES];
   const int rc = ensure_dynamic_smem(paged_chunk_kernel<T, D, MOD>, done, device, PtCfg<D>::SMEM);
   if (rc != KVB_OK) return rc;
   static_assert(PA_MAX_B * 4 <= PtCfg<D>::OFF_BAR - PtCfg<D>::OFF_KV, "the scheduler's scratch is the ring");
-  KVB_CHECK_CUDA(launch_kernel(paged_chunk_kernel<T, D, MOD>, dim3(p.grid), dim3(PT_THREADS), PtCfg<D>::SMEM, st, p));
+  CUtensorMap kmap = {}, vmap = {};
+  const int P = 1 << p.shift;
+  p.box = paged_tensor_map<T>(&kmap, p.key, p.k_sp, p.k_sh, p.k_st, D, P, p.Hkv, p.num_pages) &&
+                  paged_tensor_map<T>(&vmap, p.value, p.v_sp, p.v_sh, p.v_st, D, P, p.Hkv, p.num_pages)
+              ? (P < PT_KT ? P : PT_KT)
+              : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(PT_THREADS);
+  cfg.dynamicSmemBytes = PtCfg<D>::SMEM;
+  cfg.stream = st;
+  KVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_chunk_kernel<T, D, MOD>, p, kmap, vmap));
   if (p.grid > 1) {
     ChainLaunchScope chain;
     chain.on();

@@ -3,6 +3,8 @@
 #include "paged_common.cuh"
 #include "tcgen05.cuh"
 
+#include <cuda.h>
+
 #include <type_traits>
 
 namespace kvb {
@@ -14,43 +16,43 @@ constexpr int PT_THREADS = 512;             // warps 0-3, 4-7: softmax of row ti
 constexpr int PT_HALF = 128 * 128;          // bytes of 128 rows x 64 16-bit elements, 128-byte swizzle
 constexpr float PT_SHIFT = 7.0f;            // as in the kernel for few rows: weights reach 2^7, stale ones 2^15
 constexpr float PT_LAZY = 8.0f;
+constexpr int PT_POLY = 1;                  // of four pairs of weights, those the FMA pipe computes
 
 template <int D>
 struct PtCfg {
   static constexpr int NH = D / 64;                      // 64-element halves of a row
   static constexpr int TILEB = NH * PT_HALF;             // one 128-row operand tile
   static constexpr int ST = D == 128 ? 5 : 8;            // K/V ring stages
-  static constexpr int LAG = ST - 2 < 4 ? ST - 2 : 4;    // loads in flight behind the newest one
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILEB;
   static constexpr int OFF_BAR = OFF_KV + ST * TILEB;
   static constexpr int Q_FULL = OFF_BAR, Q_EMPTY = Q_FULL + 8, FULL = Q_EMPTY + 8, EMPTY = FULL + 8 * ST;   // barriers
-  static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 16;
+  static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 32;   // P_FULL[key half][row tile]
   static constexpr int OFF_MISC = DONE + 8;                                                             // tmem base, dead
   static constexpr int BYTES = OFF_MISC + 16;
   static constexpr int SMEM = BYTES + 1024;              // the base is brought to a swizzle atom
   static constexpr uint32_t TS = 0, TO = 256;            // tensor memory: scores at 128*w, outputs at 256 + D*w
 };
 
-__device__ __forceinline__ uint64_t pt_desc(uint32_t addr, uint32_t lbo) {
-  // 128-byte swizzle, 8-row groups 1024 bytes apart
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-         (2ull << 61);
+__device__ __forceinline__ uint64_t pt_desc(uint32_t addr16, uint32_t lbo) {
+  // address in units of 16 bytes (below 256 KiB: no carry out of its field); 128-byte swizzle, 8-row groups 1024 bytes apart
+  constexpr uint32_t hi = (1024 >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | (addr16 | (lbo >> 4) << 16);
 }
 template <typename T>
 __host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_mn_major) {
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elect) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(elect) : "memory");
 }
-__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elect) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(elect) : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t t, const uint32_t* v) {
   asm volatile(
@@ -63,19 +65,43 @@ __device__ __forceinline__ void tc_st32(uint32_t t, const uint32_t* v) {
       "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ void tc_st16(uint32_t t, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// 2^y for two finite y <= 127: y = n + f with n = rint(y) (adding 1.5 * 2^23 leaves n in the low bits), 2^f by the
+// polynomial of degree 4 with the least relative error on [-1/2, 1/2] (Remez exchange: 2.6e-6, mean 4e-8), n added to
+// the exponent. Below -125 the result stays at 2^-125, nothing next to a sum that is at least 2^-8.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t y) {
+  float a, b;
+  unpack2(y, a, b);
+  y = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
+  const float magic = 12582912.0f;
+  const uint64_t t = add2(y, pack2(magic, magic));
+  const uint64_t f = fma2(add2(t, pack2(-magic, -magic)), pack2(-1.0f, -1.0f), y);
+  uint64_t q = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
+  q = fma2(f, q, pack2(0.240247443318367f, 0.240247443318367f));
+  q = fma2(f, q, pack2(0.6931217908859253f, 0.6931217908859253f));
+  q = fma2(f, q, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb, qa, qb;
+  unpack2(t, ta, tb);
+  unpack2(q, qa, qb);
+  return pack2(__uint_as_float(__float_as_uint(qa) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(qb) + (__float_as_uint(tb) << 23)));
 }
 
 // Barriers by shared-memory address (one register instead of two).
 __device__ __forceinline__ void pt_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pt_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void pt_commit(uint32_t bar, uint32_t elect) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+               ::"r"(bar), "r"(elect) : "memory");
 }
 // Bounded wait that also gives up once another role of the block has (`dead`: a shared word).
 __device__ __forceinline__ bool pt_wait(uint32_t bar, uint32_t parity, uint32_t dead) {
@@ -116,65 +142,73 @@ struct PtPiece {
   }
 };
 
-// ---- loads: 4 warps, each 32 rows of every operand tile --------------------------------------------------
+// ---- loads: 4 warps ---------------------------------------------------------------------------------------
+// A key tile that the unit sees whole, from valid pages, is copied by the TMA engine: one box per page and 64-element
+// half, issued by the lanes of the first warp. The others (the ends of a range, a bad table entry, pages of fewer than 8
+// tokens) are copied by all four warps, 32 rows each, 16 bytes per lane, with zeros for the rows that are not seen.
 template <typename T, int D>
 struct PtLoader {
   using Cfg = PtCfg<D>;
   static constexpr int CPR = D / 8, RPI = 32 / CPR;
   const PagedParams& p;
+  const CUtensorMap* kmap;
+  const CUtensorMap* vmap;
   uint32_t base;
   int w, lane;
-  int item, sent;                                        // K/V tiles requested, and handed to the tensor core
+  int item;                                              // K/V tiles requested so far
 
-  __device__ __forceinline__ PtLoader(const PagedParams& p_, uint32_t base_, int w_, int lane_)
-      : p(p_), base(base_), w(w_), lane(lane_), item(0), sent(0) {}
+  __device__ __forceinline__ PtLoader(const PagedParams& p_, const CUtensorMap* k_, const CUtensorMap* v_, uint32_t base_, int w_,
+                                      int lane_)
+      : p(p_), kmap(k_), vmap(v_), base(base_), w(w_), lane(lane_), item(0) {}
 
   __device__ __forceinline__ void signal(uint32_t bar) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) pt_arrive(bar);
   }
-  __device__ __forceinline__ void flush() {
-    cp_async_wait<0>();
-    for (; sent < item; ++sent) signal(base + Cfg::FULL + 8 * (sent % Cfg::ST));
+  __device__ __forceinline__ bool wait_empty() {
+    return pt_wait(base + Cfg::EMPTY + 8 * (item % Cfg::ST), ((item / Cfg::ST) & 1) ^ 1, base + Cfg::OFF_MISC + 4);
   }
-  // page of this lane's row of key tile n, or -1 (row not seen by the unit, or a bad table entry)
-  __device__ __forceinline__ int page_of(const PtPiece& pc, const int32_t* table, int n) const {
-    const int t = n * PT_KT + 32 * w + lane;
-    if (n >= pc.n1 || t < pc.u.lo || t >= pc.u.hi) return -1;
-    const int page = table[t >> p.shift];
-    if (page < 0 || page >= p.num_pages) {
-      atomicExch(&g_device_status, (int)KVB_BAD_ARG);
-      return -1;
-    }
-    return page;
+  __device__ __forceinline__ uint32_t full() const { return base + Cfg::FULL + 8 * (item % Cfg::ST); }
+  __device__ __forceinline__ uint32_t stage() const { return base + Cfg::OFF_KV + (item % Cfg::ST) * Cfg::TILEB; }
+  __device__ __forceinline__ int page(const int32_t* table, int t) const {
+    const int pg = table[t >> p.shift];
+    return pg >= 0 && pg < p.num_pages ? pg : -1;
   }
-  __device__ __forceinline__ bool load_rows(const T* pool, int64_t sp, int64_t st, int n, int page) {
-    const int stage = item % Cfg::ST;
-    if (!pt_wait(base + Cfg::EMPTY + 8 * stage, ((item / Cfg::ST) & 1) ^ 1, base + Cfg::OFF_MISC + 4)) return false;
-    const uint32_t dst = base + Cfg::OFF_KV + stage * Cfg::TILEB;
-    const int c = lane % CPR, mask = (1 << p.shift) - 1;
-    const uint32_t col = dst + (c >> 3) * PT_HALF;
+  // the boxes of one key tile: `pg` is the page of this lane's box (of p.box rows)
+  __device__ __forceinline__ void load_boxes(const CUtensorMap* map, int h, int n, int pg) {
+    const uint32_t bar = full();
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)Cfg::TILEB) : "memory");
+    __syncwarp();
+    const int boxes = PT_KT / p.box;
+    if (lane < boxes) {
+      const int row = (n * PT_KT + lane * p.box) & ((1 << p.shift) - 1);
 #pragma unroll
+      for (int half = 0; half < Cfg::NH; ++half)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(stage() + half * PT_HALF + lane * p.box * 128), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(half * 64),
+            "r"(row), "r"(h), "r"(pg)
+            : "memory");
+    }
+  }
+  __device__ __forceinline__ void load_rows(const T* pool, int64_t sp, int64_t st, int n, int pg) {
+    const int c = lane % CPR, mask = (1 << p.shift) - 1;
+    const uint32_t col = stage() + (c >> 3) * PT_HALF;
+#pragma unroll 4
     for (int j = 0; j < 32 / RPI; ++j) {
       const int row = lane / CPR + j * RPI, ra = 32 * w + row;
-      const int pg = __shfl_sync(0xffffffffu, page, row);
-      const bool ok = pg >= 0;
-      const int64_t at = ok ? (int64_t)pg * sp + (int64_t)((n * PT_KT + ra) & mask) * st + c * 8 : 0;
+      const int g = __shfl_sync(0xffffffffu, pg, row);
+      const bool ok = g >= 0;
+      const int64_t at = ok ? (int64_t)g * sp + (int64_t)((n * PT_KT + ra) & mask) * st + c * 8 : 0;
       cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), pool + at, ok);
     }
     cp_async_commit();
-    ++item;
-    if (item - sent > Cfg::LAG) {
-      cp_async_wait<Cfg::LAG>();
-      signal(base + Cfg::FULL + 8 * (sent % Cfg::ST));
-      ++sent;
-    }
-    return true;
   }
   __device__ __forceinline__ void load_query(const PagedPlace& at, const PagedRequest& r) {
     const int total = r.q * p.G;
-#pragma unroll
+#pragma unroll 1
     for (int tl = 0; tl < 2; ++tl) {
       if (at.tile * PT_ROWS + tl * 128 >= total) break;
       const int flat = at.tile * PT_ROWS + tl * 128 + 32 * w + lane;
@@ -205,98 +239,156 @@ struct PtLoader {
       const int32_t* table = p.table + (int64_t)at.b * p.table_st;
       const T* kp = reinterpret_cast<const T*>(p.key) + (int64_t)at.h * p.k_sh;
       const T* vp = reinterpret_cast<const T*>(p.value) + (int64_t)at.h * p.v_sh;
-      int page = page_of(pc, table, pc.n0);
+      const int boxes = p.box > 0 ? PT_KT / p.box : 0;
+      auto box_page = [&](int n) -> int {                // the page of this lane's box of a tile seen whole
+        if (n >= pc.n1 || n * PT_KT < pc.u.lo || n * PT_KT + PT_KT > pc.u.hi || lane >= boxes) return -1;
+        return page(table, n * PT_KT + lane * p.box);
+      };
       bool ok = true;
+      int pg = box_page(pc.n0);
       for (int n = pc.n0; n < pc.n1 && ok; ++n) {
-        const int next = page_of(pc, table, n + 1);
-        ok = load_rows(kp, p.k_sp, p.k_st, n, page) && load_rows(vp, p.v_sp, p.v_st, n, page);
+        const int next = box_page(n + 1);
+        const bool whole = boxes > 0 && __all_sync(0xffffffffu, pg >= 0 || lane >= boxes) && n * PT_KT >= pc.u.lo &&
+                           n * PT_KT + PT_KT <= pc.u.hi;
+        if (whole) {
+#pragma unroll
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            if (!wait_empty()) { ok = false; break; }
+            if (w == 0) load_boxes(kv == 0 ? kmap : vmap, at.h, n, pg);
+            else if (lane == 0) pt_arrive(full());
+            ++item;
+          }
+        } else {
+          const int t = n * PT_KT + 32 * w + lane;
+          int mine = -1;
+          if (t >= pc.u.lo && t < pc.u.hi) {
+            mine = page(table, t);
+            if (mine < 0) atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+          }
+          uint32_t bar[2];
+#pragma unroll
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            if (!wait_empty()) { ok = false; break; }
+            bar[kv] = full();
+            if (kv == 0) load_rows(kp, p.k_sp, p.k_st, n, mine);
+            else load_rows(vp, p.v_sp, p.v_st, n, mine);
+            ++item;
+          }
+          if (ok) {
+            cp_async_wait<1>();
+            signal(bar[0]);
+            cp_async_wait<0>();
+            signal(bar[1]);
+          }
+        }
+        // the unit's first keys are on their way before the last unit's query is given up
         if (ok && n == pc.n0) {
-          // the next unit's first keys are on their way before the last unit's query is given up
-          flush();
           ok = pt_wait(base + Cfg::Q_EMPTY, (unit & 1) ^ 1, base + Cfg::OFF_MISC + 4);
           if (ok) load_query(at, r);
         }
-        page = next;
+        pg = next;
       }
       if (!ok) break;
       ++unit;
       left -= pc.n1 - pc.n0;
       if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
     }
-    flush();
+    cp_async_wait<0>();
   }
 };
 
-// ---- MMA issue: one thread -------------------------------------------------------------------------------
+// ---- MMA issue: one warp, one elected lane -----------------------------------------------------------------
+// Descriptors differ from a constant only in their address word. The whole warp walks the loop with values that are
+// the same in every lane (votes and shuffles say so to the compiler), so they stay in uniform registers, from which the
+// instruction takes them; with one lane inside a branch every descriptor was moved there first, and the issue loop of a
+// tile pair alone took 6000 cycles.
 template <typename T, int D>
-__device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base, uint32_t tmem, PagedPlace at, PagedRequest r, long long left) {
+__device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, uint32_t tmem_, PagedPlace at, PagedRequest r, long long left) {
   using Cfg = PtCfg<D>;
+  const uint32_t base = __shfl_sync(0xffffffffu, base_, 0), tmem = __shfl_sync(0xffffffffu, tmem_, 0);
   const uint32_t full = base + Cfg::FULL, empty = base + Cfg::EMPTY, s_full = base + Cfg::S_FULL, p_full = base + Cfg::P_FULL;
   const uint32_t dead = base + Cfg::OFF_MISC + 4;
+  const uint32_t elect = (threadIdx.x & 31) == 0 ? 1u : 0u;
   constexpr uint32_t id_s = pt_idesc<T>(PT_KT, false), id_o = pt_idesc<T>(D, true);
-  int item = 0;
+  uint32_t stage = 0, phase = 0;                         // of the next K/V tile
   uint32_t unit = 0, p_use[2] = {0, 0};
-  bool ok = true;
-  auto ring = [&](int it) { return base + Cfg::OFF_KV + (it % Cfg::ST) * Cfg::TILEB; };
-  auto scores = [&](int w, uint32_t k) {
-    const uint32_t q = base + Cfg::OFF_Q + w * Cfg::TILEB;
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, pt_wait(bar, parity, dead)); };
+  auto commit = [&](uint32_t bar) { pt_commit(bar, elect); };
+  auto step = [&]() { if (++stage == Cfg::ST) { stage = 0; phase ^= 1; } };
+  auto scores = [&](int w, uint32_t st) {
+    const uint32_t q = (base + Cfg::OFF_Q + w * Cfg::TILEB) >> 4, k = (base + Cfg::OFF_KV + st * Cfg::TILEB) >> 4;
 #pragma unroll
     for (int h = 0; h < Cfg::NH; ++h)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        pt_mma_ss(tmem + Cfg::TS + 128 * w, pt_desc(q + h * PT_HALF + s * 32, 16), pt_desc(k + h * PT_HALF + s * 32, 16), id_s,
-                  h + s > 0 ? 1u : 0u);
+        pt_mma_ss(tmem + Cfg::TS + 128 * w, pt_desc(q + ((h * PT_HALF + s * 32) >> 4), 16), pt_desc(k + ((h * PT_HALF + s * 32) >> 4), 16),
+                  id_s, h + s > 0 ? 1u : 0u, elect);
   };
-  while (ok) {
+  while (true) {
     PtPiece pc;
     pc.set(p, at, r, left);
     int na[2], nb[2];
-    pc.rows(p, at, r, 0, na[0], nb[0]);
-    pc.rows(p, at, r, 1, na[1], nb[1]);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      pc.rows(p, at, r, w, na[w], nb[w]);
+      na[w] = __shfl_sync(0xffffffffu, na[w], 0);
+      nb[w] = __shfl_sync(0xffffffffu, nb[w], 0);
+    }
+    const int n0 = __shfl_sync(0xffffffffu, pc.n0, 0), n1 = __shfl_sync(0xffffffffu, pc.n1, 0);
     // first keys and the query
-    if (!pt_wait(full + 8 * (item % Cfg::ST), (item / Cfg::ST) & 1, dead) || !pt_wait(base + Cfg::Q_FULL, unit & 1, dead)) { ok = false; break; }
+    if (!wait(full + 8 * stage, phase) || !wait(base + Cfg::Q_FULL, unit & 1)) break;
     tc_fence_after();
 #pragma unroll
     for (int w = 0; w < 2; ++w)
-      if (na[w] == pc.n0 && nb[w] > na[w]) {
-        scores(w, ring(item));
-        pt_commit(s_full + 8 * w);
+      if (na[w] == n0 && nb[w] > n0) {
+        scores(w, stage);
+        commit(s_full + 8 * w);
       }
-    pt_commit(empty + 8 * (item % Cfg::ST));
-    for (int n = pc.n0; n < pc.n1; ++n) {
-      const int v = item + 1, k = item + 2;
-      const bool more = n + 1 < pc.n1;
-      if (!pt_wait(full + 8 * (v % Cfg::ST), (v / Cfg::ST) & 1, dead) || (more && !pt_wait(full + 8 * (k % Cfg::ST), (k / Cfg::ST) & 1, dead))) {
-        ok = false;
-        break;
-      }
+    commit(empty + 8 * stage);
+    step();
+    bool ok = true;
+    for (int n = n0; n < n1; ++n) {
+      const uint32_t vs = stage, vp = phase;
+      step();
+      const uint32_t ks = stage;
+      const bool more = n + 1 < n1;
+      ok = wait(full + 8 * vs, vp) && (!more || wait(full + 8 * ks, phase));
+      if (!ok) break;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const bool pv = n >= na[w] && n < nb[w], sc = n + 1 >= na[w] && n + 1 < nb[w];
         if (pv) {
-          if (!pt_wait(p_full + 8 * w, p_use[w] & 1, dead)) { ok = false; break; }
-          ++p_use[w];
-          tc_fence_after();
+          const uint32_t v = (base + Cfg::OFF_KV + vs * Cfg::TILEB) >> 4;
 #pragma unroll
-          for (int j = 0; j < PT_KT / 16; ++j)
-            pt_mma_ts(tmem + Cfg::TO + D * w, tmem + Cfg::TS + 128 * w + 8 * j, pt_desc(ring(v) + j * 2048, PT_HALF), id_o,
-                      (n > na[w] || j > 0) ? 1u : 0u);
+          for (int half = 0; half < 2; ++half) {
+            ok = ok && wait(p_full + 16 * half + 8 * w, p_use[w] & 1);
+            if (ok) {
+              tc_fence_after();
+#pragma unroll
+              for (int j = 4 * half; j < 4 * half + 4; ++j)
+                pt_mma_ts(tmem + Cfg::TO + D * w, tmem + Cfg::TS + 128 * w + 8 * j, pt_desc(v + j * 128, PT_HALF), id_o,
+                          (n > na[w] || j > 0) ? 1u : 0u, elect);
+            }
+          }
+          ++p_use[w];
         }
-        if (sc) scores(w, ring(k));
-        if (pv || sc) pt_commit(s_full + 8 * w);
+        if (ok && sc) scores(w, ks);
+        if (ok && (pv || sc)) commit(s_full + 8 * w);
       }
       if (!ok) break;
-      pt_commit(empty + 8 * (v % Cfg::ST));
-      if (more) pt_commit(empty + 8 * (k % Cfg::ST));
-      item += 2;
+      commit(empty + 8 * vs);
+      if (more) {
+        commit(empty + 8 * ks);
+        step();
+      }
     }
     if (!ok) break;
-    pt_commit(base + Cfg::Q_EMPTY);
+    commit(base + Cfg::Q_EMPTY);
     ++unit;
-    left -= pc.n1 - pc.n0;
+    left -= n1 - n0;
     if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
   }
-  pt_commit(base + Cfg::DONE);
+  commit(base + Cfg::DONE);
   pt_wait(base + Cfg::DONE, 0, dead);
 }
 
@@ -329,38 +421,36 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       if (!pt_wait(s_full, s_use & 1, dead)) { ok = false; break; }
       ++s_use;
       tc_fence_after();
-      uint32_t v[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) TcLd<32>::ld(ts + 32 * c, v[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) TcLd<32>::wait(v[c]);
+      // Pass 1: the largest score. Scores that are changed (capped, biased, masked) go back to their place. Reading the
+      // tile twice costs less than holding its 128 scores, which leaves the other roles too few registers.
       const int t0 = n * PT_KT;
-      if constexpr (MOD) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            v[c][i] = __float_as_uint(paged_score(p, __uint_as_float(v[c][i]), slope, pos, t0 + 32 * c + i));
-      }
-      if (t0 < all_lo || t0 + PT_KT > all_hi) {
-        const uint32_t from = (uint32_t)(lo - t0), width = (uint32_t)(hi - lo);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if ((uint32_t)(32 * c + i) - from >= width) v[c][i] = 0xff800000u;
-      }
-      float mx[4];
+      const bool edge = t0 < all_lo || t0 + PT_KT > all_hi;
+      const uint32_t from = (uint32_t)(lo - t0), width = (uint32_t)(hi - lo);
+      uint32_t v[2][32];
+      float mx[2] = {-INFINITY, -INFINITY};
+      TcLd<32>::ld(ts, v[0]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(v[c][0]);
+        uint32_t* x = v[c & 1];
+        TcLd<32>::wait(x);
+        if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
+        if constexpr (MOD) paged_scores<32>(p, reinterpret_cast<float*>(x), slope, t0 + 32 * c - pos);
+        if (edge) {
 #pragma unroll
-        for (int i = 1; i < 31; i += 2)
-          asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[c]) : "f"(__uint_as_float(v[c][i])), "f"(__uint_as_float(v[c][i + 1])));
-        mx[c] = fmaxf(mx[c], __uint_as_float(v[c][31]));
+          for (int i = 0; i < 32; ++i)
+            if ((uint32_t)(32 * c + i) - from >= width) x[i] = 0xff800000u;
+        }
+        if (MOD || edge) tc_st32(ts + 32 * c, x);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[0]) : "f"(__uint_as_float(x[i])), "f"(__uint_as_float(x[i + 1])));
+          asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[1]) : "f"(__uint_as_float(x[i + 2])), "f"(__uint_as_float(x[i + 3])));
+        }
       }
+      if (MOD || edge) tc_wait_st();
+      TcLd<32>::ld(ts, v[0]);
       const float scale = MOD ? 1.0f : p.scale_log2;
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale - PT_SHIFT;
+      const float top = fmaxf(mx[0], mx[1]) * scale - PT_SHIFT;
       const bool move = top > m + PT_LAZY;
       if (__any_sync(0xffffffffu, move)) {
         const float mn = move ? top : m, a = move ? ex2(m - mn) : 1.0f;
@@ -376,29 +466,49 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
             tc_st32(to + 32 * c, o);
           }
+          TcLd<32>::ld(ts, v[0]);
         }
       }
       const float ms = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // Pass 2: weights, two at a time. PT_POLY pairs of every four come from a polynomial on the FMA pipe instead of the exponential unit,
+      // where the tile sees no mask: 16 exponentials per SM and cycle are as slow as both products together.
+      const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
+      uint64_t sum[2] = {0, 0};
+      auto weights = [&](auto poly) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          TcLd<32>::wait(v[c & 1]);
+          if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int e = 64 * c + 2 * i;
-          const float x = ex2(fmaf(__uint_as_float(v[e >> 5][e & 31]), scale, -ms));
-          const float y = ex2(fmaf(__uint_as_float(v[e >> 5][(e & 31) + 1]), scale, -ms));
-          sum[2 * (i & 1)] += x;
-          sum[2 * (i & 1) + 1] += y;
-          pk[i] = Half2Of<T>::pack(x, y);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t y = fma2(pack2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), scale2, ms2);
+            float a, b;
+            uint64_t x;
+            if (decltype(poly)::value && i % 4 < PT_POLY) {
+              x = ex2_poly2(y);
+            } else {
+              unpack2(y, a, b);
+              x = pack2(ex2(a), ex2(b));
+            }
+            sum[i & 1] = add2(sum[i & 1], x);
+            unpack2(x, a, b);
+            pk[i] = Half2Of<T>::pack(a, b);
+          }
+          tc_st16(ts + 16 * c, pk);
+          if (c & 1) {                                   // half of the keys: the second product may begin
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) pt_arrive(p_full + 16 * (c >> 1));
+          }
         }
-        tc_st32(ts + 32 * c, pk);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) pt_arrive(p_full);
+      };
+      if (edge) weights(std::false_type());
+      else weights(std::true_type());
+      float s0, s1;
+      unpack2(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
     }
     if (!ok) return;
     // ---- the unit, or this block's piece of it
@@ -451,6 +561,12 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
   }
 }
 
+// Each role walks the span with its own copy: what all three derive from it would otherwise be computed ahead of their
+// branches and held, or spilled, through all of them.
+__device__ __forceinline__ void pt_own(PagedPlace& at, PagedRequest& r, long long& left) {
+  asm volatile("" : "+r"(at.b), "+r"(at.h), "+r"(at.tile), "+r"(at.k), "+r"(r.first), "+r"(r.q), "+r"(r.kv), "+r"(r.pre), "+l"(left));
+}
+
 // A block walks its span unit by unit: 4 warps copy K and V tiles (and each unit's query rows) into shared memory in the
 // 128-byte-swizzled layout, one thread issues S_w = Q_w K^T and O_w += P_w V for two row tiles w of 128 rows, and four
 // warps per row tile, one row per thread, turn scores into weights: S_w is read from tensor memory, P_w goes back over
@@ -459,14 +575,16 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
 // 2^8, so O_w is rescaled rarely, and then by the softmax warps, which know from the order of issue that the previous
 // product is complete. Rows of K and V outside what the unit sees are zero-filled, not read.
 template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_chunk_kernel(PagedParams p) {
+__global__ void __launch_bounds__(PT_THREADS, 1)
+    paged_chunk_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using Cfg = PtCfg<D>;
   extern __shared__ uint8_t pt_raw[];
   const uint32_t raw = smem_u32(pt_raw);
   uint8_t* smem = pt_raw + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t base = smem_u32(smem);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_MISC);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in all lanes, and known to be
   pdl_launch_dependents();
 
   PagedPlace at;
@@ -490,28 +608,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_chunk_kernel(PagedParams 
     for (int w = 0; w < 2; ++w) {
       mbar_init(bar(Cfg::S_FULL + 8 * w), 1);
       mbar_init(bar(Cfg::P_FULL + 8 * w), 4);
+      mbar_init(bar(Cfg::P_FULL + 16 + 8 * w), 4);
     }
     mbar_init(bar(Cfg::DONE), 1);
     fence_mbar_init();
   }
-  const PagedRequest r = paged_request(p, at.b);
+  PagedRequest r = paged_request(p, at.b);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  // registers: 128 x 512 at launch = 192 x 256 + 64 x 256
+  // registers: 128 x 512 at launch = 160 x 256 + 64 x 128 + 128 x 128
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    pt_own(at, r, left);
     pt_softmax<T, D, MOD>(p, base, tmem, warp >> 2, tid & 127, at, r, left);
-  } else {
+  } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp < 12) {
-      PtLoader<T, D> loader(p, base, warp - 8, lane);
-      loader.run(at, r, left);
-    } else if (warp == 12 && lane == 0) {
-      pt_issue<T, D>(p, base, tmem, at, r, left);
-    }
+    pt_own(at, r, left);
+    PtLoader<T, D> loader(p, &kmap, &vmap, base, warp - 8, lane);
+    loader.run(at, r, left);
+  } else if (warp == 12) {
+    pt_own(at, r, left);
+    pt_issue<T, D>(p, base, tmem, at, r, left);
   }
   __syncwarp();
   tc_fence_before();

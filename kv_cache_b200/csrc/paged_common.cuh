@@ -41,6 +41,7 @@ struct PagedParams {
   float2* ws_ml;                                     // [2*grid][ROWS] (m, l)
   int4* ws_desc;                                     // [2*grid]: see PieceDesc
   int grid;
+  int box;                                           // rows per TMA box of a pool, 0: no TMA
 };
 
 // ws_desc[2c]: the piece that continues a unit begun by an earlier block: x = 1, y = 1 iff the unit ends in it.
@@ -245,21 +246,96 @@ __device__ __forceinline__ bool paged_next(const PagedParams& p, PagedPlace& at,
   return true;
 }
 
-// tanh without a branch: 1 - 2 / (1 + e^2y) away from zero (its rounding is relative to 1 there), the odd Taylor
-// polynomial up to y^9 below 0.35 (first term left out: 0.00886 y^10 of the value, 2.5e-7).
-__device__ __forceinline__ float paged_tanh(float y) {
-  const float e = exp2f(2.0f * PA_LOG2E * y);
-  const float big = 1.0f - __fdividef(2.0f, 1.0f + e);
-  const float z = y * y;
-  const float small = y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-  return fabsf(y) < 0.35f ? small : big;
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// The score of key j for a query at position pos, times log2(e), from the raw product q.k.
-__device__ __forceinline__ float paged_score(const PagedParams& p, float dot, float slope_log2, int pos, int j) {
-  float x = p.cap_log2 > 0.0f ? paged_tanh(dot * p.cap_in) * p.cap_log2 : dot * p.scale_log2;
-  if (p.slopes) x = fmaf(-slope_log2, fabsf((float)(pos - j)), x);
-  return x;
+// Scores of N neighbouring keys, the first at distance d0 = (key - position), in place: raw products q.k become
+// scores times log2(e). What they are made of is asked once per call, not per score.
+//
+// tanh(y) = 1 - 2 / (1 + e^2y) away from zero (its rounding is relative to 1 there); below 0.35 the odd Taylor
+// polynomial up to y^9 (first term left out: 0.00886 y^10 of the value, 2.5e-7), and where all 32 lanes' scores are that
+// small, as scores far below their cap are, the exponential is left out.
+template <int N>
+__device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, float slope_log2, int d0) {
+  if (p.cap_log2 > 0.0f) {
+    const uint64_t in2 = pack2(p.cap_in, p.cap_in), cap2 = pack2(p.cap_log2, p.cap_log2);
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t y = mul2(pack2(x[i], x[i + 1]), in2);
+      unpack2(y, x[i], x[i + 1]);
+      asm("max.f32 %0, %0, %1, %2;" : "+f"(big) : "f"(fabsf(x[i])), "f"(fabsf(x[i + 1])));
+    }
+    const bool large = __any_sync(0xffffffffu, !(big < 0.35f));
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t y = pack2(x[i], x[i + 1]);
+      const uint64_t z = mul2(y, y);
+      uint64_t q = fma2(z, pack2(62.0f / 2835.0f, 62.0f / 2835.0f), pack2(-17.0f / 315.0f, -17.0f / 315.0f));
+      q = fma2(z, q, pack2(2.0f / 15.0f, 2.0f / 15.0f));
+      q = fma2(z, q, pack2(-1.0f / 3.0f, -1.0f / 3.0f));
+      q = fma2(z, q, pack2(1.0f, 1.0f));
+      q = mul2(q, mul2(y, cap2));
+      if (large) {
+        float a, b, ya, yb;
+        unpack2(q, a, b);
+        unpack2(y, ya, yb);
+        const float ba = p.cap_log2 * fmaf(-2.0f, rcp(1.0f + ex2(ya * (2.0f * PA_LOG2E))), 1.0f);
+        const float bb = p.cap_log2 * fmaf(-2.0f, rcp(1.0f + ex2(yb * (2.0f * PA_LOG2E))), 1.0f);
+        q = pack2(fabsf(ya) < 0.35f ? a : ba, fabsf(yb) < 0.35f ? b : bb);
+      }
+      unpack2(q, x[i], x[i + 1]);
+    }
+  } else {
+    const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t y = mul2(pack2(x[i], x[i + 1]), scale2);
+      unpack2(y, x[i], x[i + 1]);
+    }
+  }
+  if (p.slopes) {
+    const uint64_t s2 = pack2(-slope_log2, -slope_log2), d2 = pack2((float)d0, (float)d0);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float a, b;
+      unpack2(add2(d2, pack2((float)i, (float)(i + 1))), a, b);
+      const uint64_t y = fma2(pack2(fabsf(a), fabsf(b)), s2, pack2(x[i], x[i + 1]));
+      unpack2(y, x[i], x[i + 1]);
+    }
+  }
 }
 
 template <typename T>
