@@ -23,10 +23,11 @@ struct PtCfg {
   static constexpr int NH = D / 64;                      // 64-element halves of a row
   static constexpr int TILEB = NH * PT_HALF;             // one 128-row operand tile
   static constexpr int ST = D == 128 ? 5 : 8;            // K/V ring stages
+  static constexpr int QS = D == 128 ? 2 : 4;            // query tiles held; with 4 the next unit's are loaded under this one
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_KV = 2 * TILEB;
+  static constexpr int OFF_KV = QS * TILEB;
   static constexpr int OFF_BAR = OFF_KV + ST * TILEB;
-  static constexpr int Q_FULL = OFF_BAR, Q_EMPTY = Q_FULL + 8, FULL = Q_EMPTY + 8, EMPTY = FULL + 8 * ST;   // barriers
+  static constexpr int Q_FULL = OFF_BAR, Q_EMPTY = Q_FULL + 8 * QS, FULL = Q_EMPTY + 8 * QS, EMPTY = FULL + 8 * ST;   // barriers
   static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 32;   // P_FULL[key half][row tile]
   static constexpr int OFF_MISC = DONE + 8;                                                             // tmem base, dead
   static constexpr int BYTES = OFF_MISC + 16;
@@ -143,9 +144,9 @@ struct PtPiece {
 };
 
 // ---- loads: 4 warps ---------------------------------------------------------------------------------------
-// A key tile that the unit sees whole, from valid pages, is copied by the TMA engine: one box per page and 64-element
-// half, issued by the lanes of the first warp. The others (the ends of a range, a bad table entry, pages of fewer than 8
-// tokens) are copied by all four warps, 32 rows each, 16 bytes per lane, with zeros for the rows that are not seen.
+// A key tile whose rows all hold tokens of the request, from valid pages, is copied by the TMA engine: one box per page
+// and 64-element half, issued by the lanes of the first warp. The others (the ends of a range, a bad table entry, pages of
+// fewer than 8 tokens) are copied by all four warps, 32 rows each, 16 bytes per lane, with zeros for the rows that are not seen.
 template <typename T, int D>
 struct PtLoader {
   using Cfg = PtCfg<D>;
@@ -156,10 +157,11 @@ struct PtLoader {
   uint32_t base;
   int w, lane;
   int item;                                              // K/V tiles requested so far
+  int rows;                                              // of them, copied row by row and not handed over yet
 
   __device__ __forceinline__ PtLoader(const PagedParams& p_, const CUtensorMap* k_, const CUtensorMap* v_, uint32_t base_, int w_,
                                       int lane_)
-      : p(p_), kmap(k_), vmap(v_), base(base_), w(w_), lane(lane_), item(0) {}
+      : p(p_), kmap(k_), vmap(v_), base(base_), w(w_), lane(lane_), item(0), rows(0) {}
 
   __device__ __forceinline__ void signal(uint32_t bar) {
     fence_proxy_async_smem();
@@ -206,90 +208,112 @@ struct PtLoader {
     }
     cp_async_commit();
   }
-  __device__ __forceinline__ void load_query(const PagedPlace& at, const PagedRequest& r) {
+  __device__ __forceinline__ uint32_t qslot(int qitem) const { return qitem % Cfg::QS; }
+  // requests the query rows of row tile tl; qitem counts the tiles
+  __device__ __forceinline__ bool load_query(const PagedPlace& at, const PagedRequest& r, int tl, int qitem) {
+    const uint32_t slot = qslot(qitem);
     const int total = r.q * p.G;
-#pragma unroll 1
-    for (int tl = 0; tl < 2; ++tl) {
-      if (at.tile * PT_ROWS + tl * 128 >= total) break;
-      const int flat = at.tile * PT_ROWS + tl * 128 + 32 * w + lane;
-      int64_t off = -1;
-      if (flat < total) {
-        const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
-        off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
-      }
-      const int c = lane % CPR;
-      const uint32_t col = base + Cfg::OFF_Q + tl * Cfg::TILEB + (c >> 3) * PT_HALF;
+    if (!pt_wait(base + Cfg::Q_EMPTY + 8 * slot, ((qitem / Cfg::QS) & 1) ^ 1, base + Cfg::OFF_MISC + 4)) return false;
+    const int flat = at.tile * PT_ROWS + tl * 128 + 32 * w + lane;
+    int64_t off = -1;
+    if (flat < total) {
+      const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
+      off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
+    }
+    const int c = lane % CPR;
+    const uint32_t col = base + Cfg::OFF_Q + slot * Cfg::TILEB + (c >> 3) * PT_HALF;
 #pragma unroll 4
-      for (int j = 0; j < 32 / RPI; ++j) {
-        const int row = lane / CPR + j * RPI, ra = 32 * w + row;
-        const int64_t o = __shfl_sync(0xffffffffu, off, row);
-        const bool ok = o >= 0;
-        cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), reinterpret_cast<const T*>(p.q) + (ok ? o + c * 8 : 0), ok);
-      }
+    for (int j = 0; j < 32 / RPI; ++j) {
+      const int row = lane / CPR + j * RPI, ra = 32 * w + row;
+      const int64_t o = __shfl_sync(0xffffffffu, off, row);
+      const bool ok = o >= 0;
+      cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), reinterpret_cast<const T*>(p.q) + (ok ? o + c * 8 : 0), ok);
     }
     cp_async_commit();
-    cp_async_wait<0>();
-    signal(base + Cfg::Q_FULL);
+    return true;
+  }
+  // Every row of the tile holds a token that the unit or a later token of the request sees: it may be copied as it is.
+  __device__ __forceinline__ bool whole(const PtPiece& pc, int kvlen, int n) const {
+    return n * PT_KT >= pc.u.lo && n * PT_KT + PT_KT <= kvlen && n * PT_KT < pc.u.hi;
+  }
+  __device__ __forceinline__ bool load_tile(const PtPiece& pc, int kvlen, int n, int h, const int32_t* table, int pg, bool boxes) {
+    if (boxes && __all_sync(0xffffffffu, pg >= 0 || lane >= PT_KT / p.box) && whole(pc, kvlen, n)) {
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        if (!wait_empty()) return false;
+        if (w == 0) load_boxes(kv == 0 ? kmap : vmap, h, n, pg);
+        else if (lane == 0) pt_arrive(full());
+        ++item;
+      }
+      return true;
+    }
+    const int t = n * PT_KT + 32 * w + lane;
+    int mine = -1;
+    if (t >= pc.u.lo && t < pc.u.hi) {
+      mine = page(table, t);
+      if (mine < 0) atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+    }
+#pragma unroll 1
+    for (int kv = 0; kv < 2; ++kv) {
+      if (!wait_empty()) return false;
+      if (kv == 0) load_rows(reinterpret_cast<const T*>(p.key) + (int64_t)h * p.k_sh, p.k_sp, p.k_st, n, mine);
+      else load_rows(reinterpret_cast<const T*>(p.value) + (int64_t)h * p.v_sh, p.v_sp, p.v_st, n, mine);
+      ++item;
+      ++rows;
+    }
+    return true;
+  }
+  // hands over what was copied row by row: `queries` row tiles from qitem on, requested before the last tile's rows
+  __device__ __forceinline__ void finish(int queries, int qitem) {
+    if (queries > 0) {
+      if (rows > 0) cp_async_wait<2>();
+      else cp_async_wait<0>();
+      for (int i = 0; i < queries; ++i) signal(base + Cfg::Q_FULL + 8 * qslot(qitem + i));
+    }
+    if (rows > 0) {
+      cp_async_wait<1>();
+      signal(base + Cfg::FULL + 8 * ((item - 2) % Cfg::ST));
+      cp_async_wait<0>();
+      signal(base + Cfg::FULL + 8 * ((item - 1) % Cfg::ST));
+      rows = 0;
+    }
   }
   __device__ __forceinline__ void run(PagedPlace at, PagedRequest r, long long left) {
-    uint32_t unit = 0;
-    while (true) {
+    int qitem = 0;
+    const bool tma = p.box > 0;
+    bool ok = true;
+    while (ok) {
       PtPiece pc;
       pc.set(p, at, r, left);
       const int32_t* table = p.table + (int64_t)at.b * p.table_st;
-      const T* kp = reinterpret_cast<const T*>(p.key) + (int64_t)at.h * p.k_sh;
-      const T* vp = reinterpret_cast<const T*>(p.value) + (int64_t)at.h * p.v_sh;
-      const int boxes = p.box > 0 ? PT_KT / p.box : 0;
       auto box_page = [&](int n) -> int {                // the page of this lane's box of a tile seen whole
-        if (n >= pc.n1 || n * PT_KT < pc.u.lo || n * PT_KT + PT_KT > pc.u.hi || lane >= boxes) return -1;
+        if (!tma || n >= pc.n1 || !whole(pc, r.kv, n) || lane >= PT_KT / p.box) return -1;
         return page(table, n * PT_KT + lane * p.box);
       };
-      bool ok = true;
       int pg = box_page(pc.n0);
+      // The unit's query and first keys are requested together. With two query slots (D = 128) the query has to wait
+      // for the last scores of the unit before this one; the first keys go ahead of it.
+      const int queries = at.tile * PT_ROWS + 128 < r.q * p.G ? 2 : 1;
+      const bool early = Cfg::QS == 4 || qitem == 0;
+      auto request = [&]() { return load_query(at, r, 0, qitem) && (queries < 2 || load_query(at, r, 1, qitem + 1)); };
+      ok = !early || request();
       for (int n = pc.n0; n < pc.n1 && ok; ++n) {
         const int next = box_page(n + 1);
-        const bool whole = boxes > 0 && __all_sync(0xffffffffu, pg >= 0 || lane >= boxes) && n * PT_KT >= pc.u.lo &&
-                           n * PT_KT + PT_KT <= pc.u.hi;
-        if (whole) {
-#pragma unroll
-          for (int kv = 0; kv < 2 && ok; ++kv) {
-            if (!wait_empty()) { ok = false; break; }
-            if (w == 0) load_boxes(kv == 0 ? kmap : vmap, at.h, n, pg);
-            else if (lane == 0) pt_arrive(full());
-            ++item;
+        ok = load_tile(pc, r.kv, n, at.h, table, pg, tma);
+        if (!ok) break;
+        if (n == pc.n0) {
+          finish(early ? queries : 0, qitem);
+          if (!early) {
+            ok = request();
+            if (ok) finish(queries, qitem);
           }
+          qitem += queries;
         } else {
-          const int t = n * PT_KT + 32 * w + lane;
-          int mine = -1;
-          if (t >= pc.u.lo && t < pc.u.hi) {
-            mine = page(table, t);
-            if (mine < 0) atomicExch(&g_device_status, (int)KVB_BAD_ARG);
-          }
-          uint32_t bar[2];
-#pragma unroll
-          for (int kv = 0; kv < 2 && ok; ++kv) {
-            if (!wait_empty()) { ok = false; break; }
-            bar[kv] = full();
-            if (kv == 0) load_rows(kp, p.k_sp, p.k_st, n, mine);
-            else load_rows(vp, p.v_sp, p.v_st, n, mine);
-            ++item;
-          }
-          if (ok) {
-            cp_async_wait<1>();
-            signal(bar[0]);
-            cp_async_wait<0>();
-            signal(bar[1]);
-          }
-        }
-        // the unit's first keys are on their way before the last unit's query is given up
-        if (ok && n == pc.n0) {
-          ok = pt_wait(base + Cfg::Q_EMPTY, (unit & 1) ^ 1, base + Cfg::OFF_MISC + 4);
-          if (ok) load_query(at, r);
+          finish(0, 0);
         }
         pg = next;
       }
       if (!ok) break;
-      ++unit;
       left -= pc.n1 - pc.n0;
       if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
     }
@@ -311,12 +335,12 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
   const uint32_t elect = (threadIdx.x & 31) == 0 ? 1u : 0u;
   constexpr uint32_t id_s = pt_idesc<T>(PT_KT, false), id_o = pt_idesc<T>(D, true);
   uint32_t stage = 0, phase = 0;                         // of the next K/V tile
-  uint32_t unit = 0, p_use[2] = {0, 0};
+  uint32_t qslot[2] = {0, 0}, qnext = 0, qphase = 0, p_use[2] = {0, 0};
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, pt_wait(bar, parity, dead)); };
   auto commit = [&](uint32_t bar) { pt_commit(bar, elect); };
   auto step = [&]() { if (++stage == Cfg::ST) { stage = 0; phase ^= 1; } };
   auto scores = [&](int w, uint32_t st) {
-    const uint32_t q = (base + Cfg::OFF_Q + w * Cfg::TILEB) >> 4, k = (base + Cfg::OFF_KV + st * Cfg::TILEB) >> 4;
+    const uint32_t q = (base + Cfg::OFF_Q + qslot[w] * Cfg::TILEB) >> 4, k = (base + Cfg::OFF_KV + st * Cfg::TILEB) >> 4;
 #pragma unroll
     for (int h = 0; h < Cfg::NH; ++h)
 #pragma unroll
@@ -335,8 +359,17 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
       nb[w] = __shfl_sync(0xffffffffu, nb[w], 0);
     }
     const int n0 = __shfl_sync(0xffffffffu, pc.n0, 0), n1 = __shfl_sync(0xffffffffu, pc.n1, 0);
+    const int tiles = __shfl_sync(0xffffffffu, at.tile * PT_ROWS + 128 < r.q * p.G ? 2 : 1, 0);
     // first keys and the query
-    if (!wait(full + 8 * stage, phase) || !wait(base + Cfg::Q_FULL, unit & 1)) break;
+    bool ok = wait(full + 8 * stage, phase);
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      if (w < tiles) {
+        ok = ok && wait(base + Cfg::Q_FULL + 8 * qnext, qphase);
+        qslot[w] = qnext;
+        if (++qnext == Cfg::QS) { qnext = 0; qphase ^= 1; }
+      }
+    if (!ok) break;
     tc_fence_after();
 #pragma unroll
     for (int w = 0; w < 2; ++w)
@@ -344,9 +377,13 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
         scores(w, stage);
         commit(s_full + 8 * w);
       }
+    if (n0 + 1 == n1) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (w < tiles) commit(base + Cfg::Q_EMPTY + 8 * qslot[w]);
+    }
     commit(empty + 8 * stage);
     step();
-    bool ok = true;
     for (int n = n0; n < n1; ++n) {
       const uint32_t vs = stage, vp = phase;
       step();
@@ -374,6 +411,7 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
         }
         if (ok && sc) scores(w, ks);
         if (ok && (pv || sc)) commit(s_full + 8 * w);
+        if (ok && n + 2 == n1 && w < tiles) commit(base + Cfg::Q_EMPTY + 8 * qslot[w]);      // these were its last scores
       }
       if (!ok) break;
       commit(empty + 8 * vs);
@@ -383,8 +421,6 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
       }
     }
     if (!ok) break;
-    commit(base + Cfg::Q_EMPTY);
-    ++unit;
     left -= n1 - n0;
     if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
   }
@@ -415,12 +451,20 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
     // keys that every row of the tile sees need no mask
     const int f0 = at.tile * PT_ROWS + w * 128;
     const int all_lo = paged_lo(r, p.window, min(r.q - 1, (f0 + 127) / p.G)), all_hi = paged_hi(r, f0 / p.G);
+    const bool any = f0 + 32 * warp < r.q * p.G;         // whether the warp has a row at all
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int n = na; n < nb; ++n) {
       if (!pt_wait(s_full, s_use & 1, dead)) { ok = false; break; }
       ++s_use;
       tc_fence_after();
+      if (!any) {                                        // what these rows weigh goes nowhere
+        if (lane == 0) {
+          pt_arrive(p_full);
+          pt_arrive(p_full + 16);
+        }
+        continue;
+      }
       // Pass 1: the largest score. Scores that are changed (capped, biased, masked) go back to their place. Reading the
       // tile twice costs less than holding its 128 scores, which leaves the other roles too few registers.
       const int t0 = n * PT_KT;
@@ -428,23 +472,36 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       const uint32_t from = (uint32_t)(lo - t0), width = (uint32_t)(hi - lo);
       uint32_t v[2][32];
       float mx[2] = {-INFINITY, -INFINITY};
-      TcLd<32>::ld(ts, v[0]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t* x = v[c & 1];
-        TcLd<32>::wait(x);
-        if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
-        if constexpr (MOD) paged_scores<32>(p, reinterpret_cast<float*>(x), slope, t0 + 32 * c - pos);
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if ((uint32_t)(32 * c + i) - from >= width) x[i] = 0xff800000u;
-        }
-        if (MOD || edge) tc_st32(ts + 32 * c, x);
+      auto largest = [&](const uint32_t* x) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[0]) : "f"(__uint_as_float(x[i])), "f"(__uint_as_float(x[i + 1])));
           asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[1]) : "f"(__uint_as_float(x[i + 2])), "f"(__uint_as_float(x[i + 3])));
+        }
+      };
+      if (MOD || edge) {
+        // a loop, not straight code: a tile would otherwise stream tens of kilobytes of instructions
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          TcLd<32>::ld(ts + 32 * c, v[0]);
+          TcLd<32>::wait(v[0]);
+          if constexpr (MOD) paged_scores<32>(p, reinterpret_cast<float*>(v[0]), slope, t0 + 32 * c - pos);
+          if (edge) {
+            const uint32_t at0 = (uint32_t)(32 * c) - from;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (at0 + i >= width) v[0][i] = 0xff800000u;
+          }
+          tc_st32(ts + 32 * c, v[0]);
+          largest(v[0]);
+        }
+      } else {
+        TcLd<32>::ld(ts, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          TcLd<32>::wait(v[c & 1]);
+          if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
+          largest(v[c & 1]);
         }
       }
       if (MOD || edge) tc_wait_st();
@@ -599,8 +656,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   if (tid == 32) {
     s_tmem[1] = 0;
     auto bar = [&](int off) { return reinterpret_cast<uint64_t*>(smem + off); };
-    mbar_init(bar(Cfg::Q_FULL), 4);
-    mbar_init(bar(Cfg::Q_EMPTY), 1);
+    for (int i = 0; i < Cfg::QS; ++i) {
+      mbar_init(bar(Cfg::Q_FULL + 8 * i), 4);
+      mbar_init(bar(Cfg::Q_EMPTY + 8 * i), 1);
+    }
     for (int i = 0; i < Cfg::ST; ++i) {
       mbar_init(bar(Cfg::FULL + 8 * i), 4);
       mbar_init(bar(Cfg::EMPTY + 8 * i), 1);
@@ -619,9 +678,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  // registers: 128 x 512 at launch = 160 x 256 + 64 x 128 + 128 x 128
+  // registers: 128 x 512 at launch = 192 x 256 + 64 x 128 + 64 x 128
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     pt_own(at, r, left);
     pt_softmax<T, D, MOD>(p, base, tmem, warp >> 2, tid & 127, at, r, left);
   } else if (warp < 12) {
@@ -629,9 +688,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     pt_own(at, r, left);
     PtLoader<T, D> loader(p, &kmap, &vmap, base, warp - 8, lane);
     loader.run(at, r, left);
-  } else if (warp == 12) {
-    pt_own(at, r, left);
-    pt_issue<T, D>(p, base, tmem, at, r, left);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 12) {
+      pt_own(at, r, left);
+      pt_issue<T, D>(p, base, tmem, at, r, left);
+    }
   }
   __syncwarp();
   tc_fence_before();

@@ -284,13 +284,14 @@ __device__ __forceinline__ float rcp(float x) {
 // Scores of N neighbouring keys, the first at distance d0 = (key - position), in place: raw products q.k become
 // scores times log2(e). What they are made of is asked once per call, not per score.
 //
-// tanh(y) = 1 - 2 / (1 + e^2y) away from zero (its rounding is relative to 1 there); below 0.35 the odd Taylor
-// polynomial up to y^9 (first term left out: 0.00886 y^10 of the value, 2.5e-7), and where all 32 lanes' scores are that
-// small, as scores far below their cap are, the exponential is left out.
+// tanh(y) = 1 - 2 / (1 + e^2y): its rounding is relative to 1, which is fp32 rounding of the largest of these scores
+// as long as that one is of the order of the cap. Where all 32 lanes' |y| are below 0.35, as scores far below their cap
+// are, the odd Taylor polynomial up to y^9 instead (first term left out: 0.00886 y^10 of the value, 2.5e-7), which also
+// leaves the exponential unit alone.
 template <int N>
 __device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, float slope_log2, int d0) {
   if (p.cap_log2 > 0.0f) {
-    const uint64_t in2 = pack2(p.cap_in, p.cap_in), cap2 = pack2(p.cap_log2, p.cap_log2);
+    const uint64_t in2 = pack2(p.cap_in, p.cap_in);
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
@@ -298,42 +299,48 @@ __device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, flo
       unpack2(y, x[i], x[i + 1]);
       asm("max.f32 %0, %0, %1, %2;" : "+f"(big) : "f"(fabsf(x[i])), "f"(fabsf(x[i + 1])));
     }
-    const bool large = __any_sync(0xffffffffu, !(big < 0.35f));
+    if (__any_sync(0xffffffffu, !(big < 0.35f))) {
+      const uint64_t two2 = pack2(2.0f * PA_LOG2E, 2.0f * PA_LOG2E), m2 = pack2(-2.0f * p.cap_log2, -2.0f * p.cap_log2);
+      const uint64_t cap2 = pack2(p.cap_log2, p.cap_log2), one2 = pack2(1.0f, 1.0f);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint64_t y = pack2(x[i], x[i + 1]);
-      const uint64_t z = mul2(y, y);
-      uint64_t q = fma2(z, pack2(62.0f / 2835.0f, 62.0f / 2835.0f), pack2(-17.0f / 315.0f, -17.0f / 315.0f));
-      q = fma2(z, q, pack2(2.0f / 15.0f, 2.0f / 15.0f));
-      q = fma2(z, q, pack2(-1.0f / 3.0f, -1.0f / 3.0f));
-      q = fma2(z, q, pack2(1.0f, 1.0f));
-      q = mul2(q, mul2(y, cap2));
-      if (large) {
-        float a, b, ya, yb;
-        unpack2(q, a, b);
-        unpack2(y, ya, yb);
-        const float ba = p.cap_log2 * fmaf(-2.0f, rcp(1.0f + ex2(ya * (2.0f * PA_LOG2E))), 1.0f);
-        const float bb = p.cap_log2 * fmaf(-2.0f, rcp(1.0f + ex2(yb * (2.0f * PA_LOG2E))), 1.0f);
-        q = pack2(fabsf(ya) < 0.35f ? a : ba, fabsf(yb) < 0.35f ? b : bb);
+      for (int i = 0; i < N; i += 2) {
+        float a, b;
+        unpack2(mul2(pack2(x[i], x[i + 1]), two2), a, b);
+        unpack2(add2(pack2(ex2(a), ex2(b)), one2), a, b);
+        unpack2(fma2(pack2(rcp(a), rcp(b)), m2, cap2), x[i], x[i + 1]);
       }
-      unpack2(q, x[i], x[i + 1]);
+    } else {
+      const uint64_t cap2 = pack2(p.cap_log2, p.cap_log2);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const uint64_t y = pack2(x[i], x[i + 1]), z = mul2(y, y);
+        uint64_t q = fma2(z, pack2(62.0f / 2835.0f, 62.0f / 2835.0f), pack2(-17.0f / 315.0f, -17.0f / 315.0f));
+        q = fma2(z, q, pack2(2.0f / 15.0f, 2.0f / 15.0f));
+        q = fma2(z, q, pack2(-1.0f / 3.0f, -1.0f / 3.0f));
+        q = fma2(z, q, pack2(1.0f, 1.0f));
+        unpack2(mul2(q, mul2(y, cap2)), x[i], x[i + 1]);
+      }
     }
   } else {
     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint64_t y = mul2(pack2(x[i], x[i + 1]), scale2);
-      unpack2(y, x[i], x[i + 1]);
-    }
+    for (int i = 0; i < N; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), scale2), x[i], x[i + 1]);
   }
   if (p.slopes) {
-    const uint64_t s2 = pack2(-slope_log2, -slope_log2), d2 = pack2((float)d0, (float)d0);
+    const uint64_t d2 = pack2((float)d0, (float)d0);
+    if (__all_sync(0xffffffffu, d0 + N <= 1)) {          // no key behind its query: |p - j| = p - j
+      const uint64_t s2 = pack2(slope_log2, slope_log2);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      float a, b;
-      unpack2(add2(d2, pack2((float)i, (float)(i + 1))), a, b);
-      const uint64_t y = fma2(pack2(fabsf(a), fabsf(b)), s2, pack2(x[i], x[i + 1]));
-      unpack2(y, x[i], x[i + 1]);
+      for (int i = 0; i < N; i += 2)
+        unpack2(fma2(add2(d2, pack2((float)i, (float)(i + 1))), s2, pack2(x[i], x[i + 1])), x[i], x[i + 1]);
+    } else {
+      const uint64_t s2 = pack2(-slope_log2, -slope_log2);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        float a, b;
+        unpack2(add2(d2, pack2((float)i, (float)(i + 1))), a, b);
+        unpack2(fma2(pack2(fabsf(a), fabsf(b)), s2, pack2(x[i], x[i + 1])), x[i], x[i + 1]);
+      }
     }
   }
 }
@@ -389,8 +396,17 @@ __global__ void __launch_bounds__(PM_WARPS * 32) paged_merge_kernel(PagedParams 
   if (blockIdx.y * PM_WARPS * RPW >= rows) return;
   // pieces: slot 2c+1, then 2(c+1), 2(c+2), ... up to the one that ends the unit
   int last = c + 1;
-  while (last < p.grid - 1 && p.ws_desc[2 * last].x != 0 && p.ws_desc[2 * last].y == 0) ++last;
-  const int n = last - c + 1;
+  while (true) {
+    const int k = last + lane;
+    const int4 e = k < p.grid ? p.ws_desc[2 * k] : make_int4(0, 1, 0, 0);
+    const unsigned stop = __ballot_sync(0xffffffffu, e.x == 0 || e.y != 0);
+    if (stop) {
+      last += __ffs(stop) - 1;
+      break;
+    }
+    last += 32;
+  }
+  const int n = min(last, p.grid - 1) - c + 1;
   for (int rr = row0; rr < min(row0 + RPW, rows); ++rr) {
     float m = -INFINITY;
     for (int s = lane; s < n; s += 32) m = fmaxf(m, p.ws_ml[(int64_t)(s == 0 ? 2 * c + 1 : 2 * (c + s)) * ROWS + rr].x);

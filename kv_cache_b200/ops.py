@@ -31,6 +31,11 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _raw_stream(index: int) -> int:
+    """The current stream of device ``index`` as an address, without making a Stream object (4 us of a 20 us call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _dev(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise RuntimeError("kv_cache_b200 operators need CUDA tensors; there is no CPU path")
@@ -753,25 +758,23 @@ class PagePlan:
     status: torch.Tensor        # int32 [4] all 0, or why nothing was planned (see page_plan)
 
 
-def _device_ints(name: str, t: torch.Tensor, n: Optional[int], device: torch.device, dtype=torch.int32) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
-        raise RuntimeError(f"{name} must be a dense {str(dtype).split('.')[-1]} vector" + ("" if n is None else f" of {n}"))
-    if t.device != device:
-        raise RuntimeError(f"{name} must be on {device}")
-    return t
+def _device_ints(name: str, t: torch.Tensor, n: int, index: int, dtype=torch.int32) -> None:
+    if t.dtype != dtype or t.dim() != 1 or (n >= 0 and t.shape[0] != n) or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a dense {str(dtype).split('.')[-1]} vector" + ("" if n < 0 else f" of {n}"))
+    if t.get_device() != index:
+        raise RuntimeError(f"{name} must be on the same device as the other operands")
 
 
-def _check_page_table(page_table: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1 \
-            or page_table.stride(1) != 1 or (batch > 1 and page_table.stride(0) < page_table.shape[1]):
+def _check_page_table(page_table: torch.Tensor, batch: int, index: int) -> int:
+    """Checks int32 ``[B,W]`` with dense rows; returns the row stride."""
+    if page_table.dtype != torch.int32 or page_table.dim() != 2:
         raise RuntimeError("page_table must be int32 [B, pages] with dense rows")
-    if page_table.device != device:
-        raise RuntimeError(f"page_table must be on {device}")
-    return page_table
-
-
-def _table_stride(page_table: torch.Tensor) -> int:
-    return max(page_table.stride(0), page_table.shape[1])
+    (B, W), (s0, s1) = page_table.shape, page_table.stride()
+    if B != batch or W < 1 or (s1 != 1 and W > 1) or (B > 1 and s0 < W):
+        raise RuntimeError("page_table must be int32 [B, pages] with dense rows")
+    if page_table.get_device() != index:
+        raise RuntimeError("page_table must be on the same device as the other operands")
+    return max(s0, W)
 
 
 def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
@@ -787,29 +790,32 @@ def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tenso
 
     ``status`` of the result: pages lacking, tokens beyond ``capacity``, requests whose table row is too short, 1 if
     the stack or a finished length cannot be. Unless all are 0 nothing is changed and no token has a slot."""
-    dev = kv_len.device
+    dev = kv_len.get_device()
     B = kv_len.shape[0] if kv_len.dim() == 1 else -1
     if B < 1 or B > 8192:
         raise RuntimeError("page_plan takes 1 to 8192 requests")
     _device_ints("kv_len", kv_len, B, dev)
     _device_ints("q_len", q_len, B, dev)
-    _check_page_table(page_table, B, dev)
-    _device_ints("free_pages", free_pages, None, dev)
+    table_stride = _check_page_table(page_table, B, dev)
+    _device_ints("free_pages", free_pages, -1, dev)
     _device_ints("free_count", free_count, 1, dev)
+    page_tokens, capacity = int(page_tokens), int(capacity)
     if page_tokens < 1 or page_tokens & (page_tokens - 1):
         raise RuntimeError("page_tokens must be a power of two")
     if capacity < 1 or free_pages.shape[0] < 1:
         raise RuntimeError("capacity and the number of pages must be positive")
     if finished is not None:
         if finished.dtype not in (torch.bool, torch.uint8) or finished.shape != (B,) or not finished.is_contiguous() \
-                or finished.device != dev:
+                or finished.get_device() != dev:
             raise RuntimeError("finished must be a dense bool or uint8 vector, one element per request")
+    if dev < 0:
+        _dev(kv_len)
     if out is None:
-        i32 = dict(dtype=torch.int32, device=dev)
-        out = PagePlan(torch.empty(B + 1, **i32), kv_len if in_place else torch.empty(B, **i32),
-                       free_count if in_place else torch.empty(1, **i32),
-                       torch.empty(capacity, dtype=torch.int64, device=dev), torch.empty(capacity, **i32),
-                       torch.empty(capacity, **i32), torch.empty(4, **i32))
+        # one allocation for the 32-bit outputs: a step's plan is made once and short
+        ints = torch.empty(2 * B + 6 + 2 * capacity, dtype=torch.int32, device=kv_len.device)
+        cu, now, left, pos, req, status = ints.split((B + 1, B, 1, capacity, capacity, 4))
+        slot = torch.empty(capacity, dtype=torch.int64, device=kv_len.device)
+        out = PagePlan(cu, kv_len if in_place else now, free_count if in_place else left, slot, pos, req, status)
     else:
         if in_place and (out.kv_len is not kv_len or out.free_count is not free_count):
             raise RuntimeError("in_place needs the plan's own kv_len and free_count")
@@ -818,26 +824,35 @@ def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tenso
             _device_ints(name, getattr(out, name), n, dev)
         _device_ints("slot", out.slot, capacity, dev, torch.int64)
     check(_native.lib().kvb_page_plan(
-        kv_len.data_ptr(), q_len.data_ptr(), _ptr(finished), B, page_table.data_ptr(), _table_stride(page_table),
-        page_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), int(page_tokens), int(capacity),
-        out.cu_q.data_ptr(), out.kv_len.data_ptr(), out.free_count.data_ptr(), out.slot.data_ptr(), out.position.data_ptr(),
-        out.request.data_ptr(), out.status.data_ptr(), _dev(kv_len), _stream(dev)), "kvb_page_plan")
+        kv_len.data_ptr(), q_len.data_ptr(), None if finished is None else finished.data_ptr(), B, page_table.data_ptr(),
+        table_stride, page_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_tokens,
+        capacity, out.cu_q.data_ptr(), out.kv_len.data_ptr(), out.free_count.data_ptr(), out.slot.data_ptr(),
+        out.position.data_ptr(), out.request.data_ptr(), out.status.data_ptr(), dev, _raw_stream(dev)), "kvb_page_plan")
     return out
 
 
-def _check_pools(key_pool: torch.Tensor, value_pool: torch.Tensor, device: torch.device) -> None:
-    if key_pool.dim() != 4 or value_pool.shape != key_pool.shape or value_pool.dtype != key_pool.dtype:
+def _check_pools(key_pool: torch.Tensor, value_pool: torch.Tensor, index: int):
+    """Checks two page pools; returns their shape and strides."""
+    shape = key_pool.shape
+    if len(shape) != 4 or value_pool.shape != shape or value_pool.dtype != key_pool.dtype:
         raise RuntimeError("key_pool and value_pool must be [num_pages,Hkv,page_tokens,D] of equal shape and type")
-    if key_pool.dtype not in (torch.bfloat16, torch.float16):
+    if key_pool.dtype != torch.bfloat16 and key_pool.dtype != torch.float16:
         raise RuntimeError("pools must be bf16 or fp16")
-    P = key_pool.shape[2]
-    if P < 1 or P & (P - 1):
+    if shape[2] < 1 or shape[2] & (shape[2] - 1):
         raise RuntimeError("page_tokens must be a power of two")
-    for t in (key_pool, value_pool):
-        if t.device != device:
-            raise RuntimeError(f"pools must be on {device}")
-        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
-            raise RuntimeError("pool rows must be contiguous and 16-byte aligned, strides multiples of 8 elements")
+    if key_pool.get_device() != index or value_pool.get_device() != index:
+        raise RuntimeError("pools must be on the same device as the other operands")
+    ks, vs = key_pool.stride(), value_pool.stride()
+    if ks[3] != 1 or vs[3] != 1 or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7 \
+            or (key_pool.data_ptr() | value_pool.data_ptr()) & 15:
+        raise RuntimeError("pool rows must be contiguous and 16-byte aligned, strides multiples of 8 elements")
+    return shape, ks, vs
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """``[N,H,D]`` with contiguous D and 16-byte aligned rows, copied only when it is not."""
+    s = t.stride()
+    return t if s[2] == 1 and not (s[0] | s[1]) & 7 and not t.data_ptr() & 15 else t.contiguous()
 
 
 def paged_append(key_rows: torch.Tensor, value_rows: torch.Tensor, slot: torch.Tensor, key_pool: torch.Tensor,
@@ -845,24 +860,25 @@ def paged_append(key_rows: torch.Tensor, value_rows: torch.Tensor, slot: torch.T
     """Stores new K and V rows ``[N,Hkv,D]`` (any token and head strides) at their ``slot`` (int64 ``[N]`` of
     ``page_plan``) in the pools ``[num_pages,Hkv,page_tokens,D]``; rows whose slot is -1 are skipped. A slot that
     appears twice receives one of its rows, which one is not defined."""
-    dev = key_pool.device
+    dev = key_pool.get_device()
     if key_rows.dim() != 3 or value_rows.shape != key_rows.shape:
         raise RuntimeError("key_rows and value_rows must be [N,Hkv,D] of equal shape")
-    _check_pools(key_pool, value_pool, dev)
-    num_pages, Hkv, P, D = key_pool.shape
-    if key_rows.shape[1:] != (Hkv, D) or key_rows.dtype != key_pool.dtype or value_rows.dtype != key_pool.dtype:
+    (num_pages, Hkv, P, D), ks, vs = _check_pools(key_pool, value_pool, dev)
+    N, H, Dr = key_rows.shape
+    if H != Hkv or Dr != D or key_rows.dtype != key_pool.dtype or value_rows.dtype != key_pool.dtype:
         raise RuntimeError("rows and pools must have the same heads, head size and type")
-    if key_rows.device != dev or value_rows.device != dev:
-        raise RuntimeError(f"rows must be on {dev}")
-    N = key_rows.shape[0]
+    if key_rows.get_device() != dev or value_rows.get_device() != dev:
+        raise RuntimeError("rows must be on the same device as the pools")
     _device_ints("slot", slot, N, dev, torch.int64)
+    if dev < 0:
+        _dev(key_pool)
     if N == 0:
         return
-    k, v = _rows_contiguous(key_rows), _rows_contiguous(value_rows)
+    k, v = _aligned_rows(key_rows), _aligned_rows(value_rows)
+    (k0, k1, _), (v0, v1, _) = k.stride(), v.stride()
     check(_native.lib().kvb_paged_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slot.data_ptr(), N, Hkv, D,
-        key_pool.data_ptr(), *key_pool.stride()[:3], value_pool.data_ptr(), *value_pool.stride()[:3], num_pages, P,
-        _dev(key_pool), _stream(dev)), "kvb_paged_append")
+        k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, slot.data_ptr(), N, Hkv, D, key_pool.data_ptr(), ks[0], ks[1], ks[2],
+        value_pool.data_ptr(), vs[0], vs[1], vs[2], num_pages, P, dev, _raw_stream(dev)), "kvb_paged_append")
 
 
 def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
@@ -881,13 +897,13 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     ``return_lse`` also returns the fp32 ``[N,Hq]`` logarithm of each row's sum of exponentials. A row that sees no key
     is zero, its logarithm -inf. ``max_q``: the largest number of new tokens of one request when the caller knows it;
     it chooses the kernel and never the result. K and V rows that some token of their request sees must be finite."""
-    dev = query.device
+    dev = query.get_device()
     if query.dim() != 3:
         raise RuntimeError("query must be [N,Hq,D]")
-    _check_pools(key_pool, value_pool, dev)
+    (num_pages, Hkv, P, Dk), ks, vs = _check_pools(key_pool, value_pool, dev)
     N, Hq, D = query.shape
-    num_pages, Hkv, P, Dk = key_pool.shape
-    if query.dtype != key_pool.dtype:
+    dtype = query.dtype
+    if dtype != key_pool.dtype:
         raise RuntimeError("query and pools must have the same type")
     if Dk != D or D not in (64, 128):
         raise RuntimeError("head size must be 64 or 128, the same for query and pools")
@@ -897,7 +913,7 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     if B < 1 or B > 8192:
         raise RuntimeError("paged_attend takes 1 to 8192 requests")
     _device_ints("kv_len", kv_len, B, dev)
-    _check_page_table(page_table, B, dev)
+    table_stride = _check_page_table(page_table, B, dev)
     if cu_q is not None:
         _device_ints("cu_q", cu_q, B + 1, dev)
     elif N != B:
@@ -907,35 +923,35 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     if slopes is not None:
         _device_ints("slopes", slopes, Hq, dev, torch.float32)
     scaling = float(D) ** -0.5 if scaling is None else float(scaling)
+    softcap, window, max_q = float(softcap), int(window), int(max_q)
     if not 0.0 < scaling < 3.0e38 or not 0.0 <= softcap < 3.0e38 or window < 0 or max_q < 0:
         raise RuntimeError("scaling must be positive and finite, softcap, window and max_q not negative")
-    query = _rows_contiguous(query)
-    if out is None:
-        out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
-    elif out.shape != (N, Hq, D) or out.dtype != query.dtype or not out.is_contiguous() or out.device != dev \
-            or out.data_ptr() % 16:
+    if out is not None and (out.shape != query.shape or out.dtype != dtype or not out.is_contiguous()
+                            or out.get_device() != dev or out.data_ptr() & 15):
         raise RuntimeError("out must be a dense, 16-byte aligned tensor of the query's shape and type")
-    lse = torch.empty((N, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if dev < 0:
+        _dev(query)
+    query = _aligned_rows(query)
+    device = query.device
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=dtype, device=device)
+    lse = torch.empty((N, Hq), dtype=torch.float32, device=device) if return_lse else None
     if N == 0:
         return (out, lse) if return_lse else out
     lib = _native.lib()
     W = page_table.shape[1]
-    ws_bytes = lib.kvb_paged_attend_workspace_bytes(N, B, Hq, Hkv, W, P, D, int(max_q))
+    ws_bytes = lib.kvb_paged_attend_workspace_bytes(N, B, Hq, Hkv, W, P, D, max_q)
     if ws_bytes == 0:
         raise RuntimeError("kvb_paged_attend: unsupported shape")
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    p = PagedAttendParams()
-    p.query, p.q_st, p.q_sh = query.data_ptr(), query.stride(0), query.stride(1)
-    p.key_pool, p.k_sp, p.k_sh, p.k_st = key_pool.data_ptr(), *key_pool.stride()[:3]
-    p.value_pool, p.v_sp, p.v_sh, p.v_st = value_pool.data_ptr(), *value_pool.stride()[:3]
-    p.page_table, p.page_table_stride = page_table.data_ptr(), _table_stride(page_table)
-    p.kv_len, p.cu_q, p.prefix_len, p.slopes = kv_len.data_ptr(), _ptr(cu_q), _ptr(prefix_len), _ptr(slopes)
-    p.elem_type = 0 if query.dtype == torch.bfloat16 else 1
-    p.N, p.B, p.Hq, p.Hkv, p.D, p.W, p.num_pages, p.page_tokens = N, B, Hq, Hkv, D, W, num_pages, P
-    p.max_q, p.window, p.scaling, p.softcap = int(max_q), int(window), scaling, float(softcap)
-    p.out, p.lse = out.data_ptr(), _ptr(lse)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), ws_bytes
-    check(lib.kvb_paged_attend(C.byref(p), _dev(query), _stream(dev)), "kvb_paged_attend")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    q0, q1, _ = query.stride()
+    p = PagedAttendParams(                               # in the order of the struct
+        query.data_ptr(), q0, q1, key_pool.data_ptr(), ks[0], ks[1], ks[2], value_pool.data_ptr(), vs[0], vs[1], vs[2],
+        page_table.data_ptr(), table_stride, kv_len.data_ptr(), None if cu_q is None else cu_q.data_ptr(),
+        None if prefix_len is None else prefix_len.data_ptr(), None if slopes is None else slopes.data_ptr(),
+        0 if dtype == torch.bfloat16 else 1, N, B, Hq, Hkv, D, W, num_pages, P, max_q, window, scaling, softcap,
+        out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws_bytes)
+    check(lib.kvb_paged_attend(C.byref(p), dev, _raw_stream(dev)), "kvb_paged_attend")
     return (out, lse) if return_lse else out
 
 
