@@ -9,6 +9,7 @@ constexpr int PR_THREADS = PR_WARPS * 32;
 constexpr int PR_ROWS = 16;                 // rows of a unit: one mma A tile
 constexpr int PR_KT = 16 * PR_WARPS;        // keys of a tile, 16 per warp
 constexpr int PR_STAGES = 3;
+constexpr int PR_SNAP = 1, PR_LEAST = 2;    // key tiles: see paged_common.cuh
 constexpr int PR_MAX_GRID = 296;            // two blocks per SM
 constexpr float PR_SHIFT = 7.0f;            // the reference of a row lies 2^7 above zero weight: fresh weights reach
 constexpr float PR_LAZY = 8.0f;             // 2^7, stale ones 2^15, inside fp16's range; small ones keep its normal bits
@@ -49,11 +50,10 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
   const int g = lane >> 2, t4 = lane & 3;
   pdl_launch_dependents();
 
-  PagedPlace at;
-  long long left;
-  paged_span<PR_ROWS, PR_KT, PR_THREADS>(p, reinterpret_cast<int*>(pr_smem), at, left, 2);
-  if (threadIdx.x < 2) p.ws_desc[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
-  if (left <= 0) return;
+  PagedSpan span = paged_span<PR_ROWS, PR_KT, PR_THREADS>(p, reinterpret_cast<int*>(pr_smem), PR_SNAP, PR_LEAST);
+  if (threadIdx.x == 0) p.ws_desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (span.left <= 0) return;
+  PagedPlace& at = span.at;
   PagedRequest r = paged_request(p, at.b);
 
   uint8_t* my = pr_smem + warp * Cfg::WARPB;
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
   while (true) {
     PagedUnit<PR_ROWS, PR_KT> u;
     u.set(r, p.G, p.window, at.tile);
-    const int ntile = (int)min((long long)(u.n - at.k), left);
+    const int ntile = (int)min((long long)(u.n - at.k), span.left);
     const bool begins = at.k == 0, ends = at.k + ntile == u.n;
     const int rows = min(PR_ROWS, r.q * p.G - at.tile * PR_ROWS);
     const int key0 = (u.t0 + at.k) * PR_KT + warp * 16;
@@ -290,10 +290,13 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
         if (lane == 0) p.ws_ml[(int64_t)slot * PR_ROWS + row] = make_float2(M, L);
       }
     }
-    if (!(begins && ends) && threadIdx.x == 0)
-      p.ws_desc[slot] = begins ? make_int4(1, at.b, at.h, at.tile) : make_int4(1, ends ? 1 : 0, 0, 0);
-    left -= ntile;
-    if (left <= 0 || !paged_next<PR_ROWS>(p, at, r)) break;
+    if (begins && !ends && threadIdx.x == 0) {
+      p.ws_desc[2 * blockIdx.x] = make_int4(paged_pieces(span.per, span.x, u.n, PR_SNAP, blockIdx.x), at.h, at.tile, 0);
+      p.ws_desc[2 * blockIdx.x + 1] = make_int4(r.first, r.q, 0, 0);
+    }
+    span.left -= ntile;
+    span.x += ntile;
+    if (span.left <= 0 || !paged_next<PR_ROWS>(p, at, r)) break;
     __syncthreads();                                     // the ring is read no more
   }
 }
@@ -306,7 +309,7 @@ static inline int64_t paged_tile_bound(int64_t N, int B, int Hkv, int G, int64_t
 static inline bool paged_few_rows(int N, int B, int G, int max_q) {
   return (int64_t)(max_q > 0 ? max_q : N == B ? 1 : N) * G <= PR_ROWS;
 }
-struct PagedSizes { bool few; int grid, rows; };
+struct PagedSizes { bool few; int grid, rows, few_tiles; };
 static inline PagedSizes paged_sizes(int N, int B, int Hkv, int G, int64_t keys, int max_q) {
   PagedSizes s;
   s.few = paged_few_rows(N, B, G, max_q);
@@ -314,6 +317,7 @@ static inline PagedSizes paged_sizes(int N, int B, int Hkv, int G, int64_t keys,
   const int64_t most = s.few ? PR_MAX_GRID : PT_MAX_GRID;
   const int64_t t = paged_tile_bound(N, B, Hkv, G, keys, s.rows, s.few ? PR_KT : PT_KT);
   s.grid = (int)(t < most ? t : most);
+  s.few_tiles = t < 0x7fffffff;
   return s;
 }
 static inline size_t paged_ws_bytes(int grid, int rows, int D) {
@@ -338,11 +342,11 @@ static int launch_paged_rows(PagedParams& p, int device, cudaStream_t st) {
   return KVB_OK;
 }
 
-// The pool as a 4-D tensor (element of a row, row of a page, KV head, page) in boxes of 64 elements x min(page, 128)
-// rows, 128-byte swizzle: the layout the tensor core reads. False when the driver takes no such map (a stride of 0, or
-// beyond its range); rows are then copied one by one.
+// A tensor of `rank` dimensions (the first contiguous) in boxes of 64 elements, 128-byte swizzle: the layout the tensor
+// core reads. False when the driver takes no such map (a stride of 0 or beyond its range); rows are copied one by one then.
 template <typename T>
-static bool paged_tensor_map(CUtensorMap* map, const void* pool, int64_t sp, int64_t sh, int64_t st, int D, int P, int Hkv, int pages) {
+static bool paged_tensor_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const int64_t* strides,
+                             const cuuint32_t* box) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -352,14 +356,17 @@ static bool paged_tensor_map(CUtensorMap* map, const void* pool, int64_t sp, int
     if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess) fn = nullptr;
     return reinterpret_cast<Encode>(fn);
   }();
-  if (!encode || P < 8 || st < D || (Hkv > 1 && sh < D) || (pages > 1 && sp < D)) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)P, (cuuint64_t)Hkv, (cuuint64_t)pages};
-  // a dimension of one element has no stride of its own
-  const cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)(Hkv > 1 ? sh : D) * 2, (cuuint64_t)(pages > 1 ? sp : D) * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)(P < PT_KT ? P : PT_KT), 1, 1}, step[4] = {1, 1, 1, 1};
-  return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  if (!encode) return false;
+  cuuint64_t bytes[3];
+  for (int i = 0; i + 1 < rank; ++i) {
+    const int64_t s = dims[i + 1] > 1 ? strides[i] : (int64_t)dims[0];      // a dimension of one element has no stride of its own
+    if (s < (int64_t)dims[0]) return false;
+    bytes[i] = (cuuint64_t)s * 2;
+  }
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                (cuuint32_t)rank, const_cast<void*>(base), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int D, bool MOD>
@@ -368,18 +375,22 @@ static int launch_paged_chunk(PagedParams& p, int device, cudaStream_t st) {
   const int rc = ensure_dynamic_smem(paged_chunk_kernel<T, D, MOD>, done, device, PtCfg<D>::SMEM);
   if (rc != KVB_OK) return rc;
   static_assert(PA_MAX_B * 4 <= PtCfg<D>::OFF_BAR - PtCfg<D>::OFF_KV, "the scheduler's scratch is the ring");
-  CUtensorMap kmap = {}, vmap = {};
-  const int P = 1 << p.shift;
-  p.box = paged_tensor_map<T>(&kmap, p.key, p.k_sp, p.k_sh, p.k_st, D, P, p.Hkv, p.num_pages) &&
-                  paged_tensor_map<T>(&vmap, p.value, p.v_sp, p.v_sh, p.v_st, D, P, p.Hkv, p.num_pages)
-              ? (P < PT_KT ? P : PT_KT)
-              : 0;
+  CUtensorMap kmap = {}, vmap = {}, qmap = {};
+  const int P = 1 << p.shift, box = P < PT_KT ? P : PT_KT;
+  const cuuint64_t pool[4] = {(cuuint64_t)D, (cuuint64_t)P, (cuuint64_t)p.Hkv, (cuuint64_t)p.num_pages};
+  const int64_t ks[3] = {p.k_st, p.k_sh, p.k_sp}, vs[3] = {p.v_st, p.v_sh, p.v_sp};
+  const cuuint32_t rows[4] = {64, (cuuint32_t)box, 1, 1};
+  p.box = P >= 8 && paged_tensor_map<T>(&kmap, p.key, 4, pool, ks, rows) && paged_tensor_map<T>(&vmap, p.value, 4, pool, vs, rows) ? box : 0;
+  const cuuint64_t query[3] = {(cuuint64_t)D, (cuuint64_t)p.Hq, (cuuint64_t)p.N};
+  const int64_t qs[2] = {p.q_sh, p.q_st};
+  const cuuint32_t tokens[3] = {64, (cuuint32_t)p.G, (cuuint32_t)(128 / p.G)};
+  p.qbox = p.G <= 128 && 128 % p.G == 0 && paged_tensor_map<T>(&qmap, p.q, 3, query, qs, tokens) ? 128 / p.G : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.grid);
   cfg.blockDim = dim3(PT_THREADS);
   cfg.dynamicSmemBytes = PtCfg<D>::SMEM;
   cfg.stream = st;
-  KVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_chunk_kernel<T, D, MOD>, p, kmap, vmap));
+  KVB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_chunk_kernel<T, D, MOD>, p, kmap, vmap, qmap));
   if (p.grid > 1) {
     ChainLaunchScope chain;
     chain.on();
@@ -456,6 +467,7 @@ extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb
   p.out = a->out; p.lse = a->lse;
   const PagedSizes s = paged_sizes(a->N, a->B, a->Hkv, p.G, keys, a->max_q);
   p.grid = s.grid;
+  p.few_tiles = s.few_tiles;
   if (a->workspace_bytes < paged_ws_bytes(s.grid, s.rows, a->D)) return KVB_WORKSPACE_TOO_SMALL;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.ws_o = reinterpret_cast<float*>(ws);

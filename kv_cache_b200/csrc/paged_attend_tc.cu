@@ -11,12 +11,12 @@ namespace kvb {
 
 constexpr int PT_ROWS = 256;                // rows of a unit: two accumulator tiles of 128
 constexpr int PT_MAX_GRID = 148;            // one block per SM
+constexpr int PT_SNAP = 2, PT_LEAST = 3;    // key tiles: see paged_common.cuh
 constexpr int PT_KT = 128;                  // keys per tile
-constexpr int PT_THREADS = 512;             // warps 0-3, 4-7: softmax of row tile 0, 1; 8-11: loads; 12: MMA issue
+constexpr int PT_THREADS = 384;             // warps 0-3, 4-7: softmax of row tile 0, 1; 8, 9: loads; 10: MMA issue
 constexpr int PT_HALF = 128 * 128;          // bytes of 128 rows x 64 16-bit elements, 128-byte swizzle
 constexpr float PT_SHIFT = 7.0f;            // as in the kernel for few rows: weights reach 2^7, stale ones 2^15
 constexpr float PT_LAZY = 8.0f;
-constexpr int PT_POLY = 1;                  // of four pairs of weights, those the FMA pipe computes
 
 template <int D>
 struct PtCfg {
@@ -28,9 +28,9 @@ struct PtCfg {
   static constexpr int OFF_KV = QS * TILEB;
   static constexpr int OFF_BAR = OFF_KV + ST * TILEB;
   static constexpr int Q_FULL = OFF_BAR, Q_EMPTY = Q_FULL + 8 * QS, FULL = Q_EMPTY + 8 * QS, EMPTY = FULL + 8 * ST;   // barriers
-  static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 32;   // P_FULL[key half][row tile]
-  static constexpr int OFF_MISC = DONE + 8;                                                             // tmem base, dead
-  static constexpr int BYTES = OFF_MISC + 16;
+  static constexpr int S_FULL = EMPTY + 8 * ST, P_FULL = S_FULL + 16, DONE = P_FULL + 32, GO = DONE + 8;   // P_FULL[key half][row tile]
+  static constexpr int OFF_MISC = GO + 8;                                                             // tmem base, dead
+  static constexpr int BYTES = OFF_MISC + 16;           // the third word stays 0: a wait that must not be cut short
   static constexpr int SMEM = BYTES + 1024;              // the base is brought to a swizzle atom
   static constexpr uint32_t TS = 0, TO = 256;            // tensor memory: scores at 128*w, outputs at 256 + D*w
 };
@@ -45,15 +45,15 @@ __host__ __device__ constexpr uint32_t pt_idesc(int n, bool b_mn_major) {
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elect) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(elect) : "memory");
+__device__ __forceinline__ void pt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
-__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elect) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(elect) : "memory");
+__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 __device__ __forceinline__ void tc_st32(uint32_t t, const uint32_t* v) {
   asm volatile(
@@ -75,44 +75,32 @@ __device__ __forceinline__ void tc_st16(uint32_t t, const uint32_t* v) {
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 2^y for two finite y <= 127: y = n + f with n = rint(y) (adding 1.5 * 2^23 leaves n in the low bits), 2^f by the
-// polynomial of degree 4 with the least relative error on [-1/2, 1/2] (Remez exchange: 2.6e-6, mean 4e-8), n added to
-// the exponent. Below -125 the result stays at 2^-125, nothing next to a sum that is at least 2^-8.
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t y) {
-  float a, b;
-  unpack2(y, a, b);
-  y = pack2(fmaxf(a, -125.0f), fmaxf(b, -125.0f));
-  const float magic = 12582912.0f;
-  const uint64_t t = add2(y, pack2(magic, magic));
-  const uint64_t f = fma2(add2(t, pack2(-magic, -magic)), pack2(-1.0f, -1.0f), y);
-  uint64_t q = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
-  q = fma2(f, q, pack2(0.240247443318367f, 0.240247443318367f));
-  q = fma2(f, q, pack2(0.6931217908859253f, 0.6931217908859253f));
-  q = fma2(f, q, pack2(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb, qa, qb;
-  unpack2(t, ta, tb);
-  unpack2(q, qa, qb);
-  return pack2(__uint_as_float(__float_as_uint(qa) + (__float_as_uint(ta) << 23)), __uint_as_float(__float_as_uint(qb) + (__float_as_uint(tb) << 23)));
-}
-
 // Barriers by shared-memory address (one register instead of two).
 __device__ __forceinline__ void pt_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pt_commit(uint32_t bar, uint32_t elect) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-               ::"r"(bar), "r"(elect) : "memory");
+__device__ __forceinline__ void pt_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// Bounded wait that also gives up once another role of the block has (`dead`: a shared word).
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool pt_elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one)::"memory");
+  return one != 0;
+}
+// Wait of at most two seconds that also ends once another role of the block has given up (`dead`: a shared word).
 __device__ __forceinline__ bool pt_wait(uint32_t bar, uint32_t parity, uint32_t dead) {
-  for (uint32_t i = 0; i < (1u << 22); ++i) {
-    uint32_t ok;
+  uint32_t ok, began = 0;
+  for (uint32_t i = 0;; ++i) {
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (ok) return true;
     asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(ok) : "r"(dead) : "memory");
     if (ok) return false;
+    uint32_t now;
+    asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(now));
+    if (i == 0) began = now;
+    else if (now - began > 2000000000u) break;
   }
   asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(dead), "r"(1u) : "memory");
   atomicExch(&g_device_status, (int)KVB_TIMEOUT);
@@ -143,10 +131,12 @@ struct PtPiece {
   }
 };
 
-// ---- loads: 4 warps ---------------------------------------------------------------------------------------
-// A key tile whose rows all hold tokens of the request, from valid pages, is copied by the TMA engine: one box per page
-// and 64-element half, issued by the lanes of the first warp. The others (the ends of a range, a bad table entry, pages of
-// fewer than 8 tokens) are copied by all four warps, 32 rows each, 16 bytes per lane, with zeros for the rows that are not seen.
+// ---- loads: 2 warps ---------------------------------------------------------------------------------------
+// The first warp copies by TMA what can be copied as it is: key tiles whose rows all hold tokens of the request, one box
+// per page and 64-element half (a page id out of range: a box beyond the pool, which the engine fills with zeros), and
+// query tiles when the heads of a KV head divide 128 (a box of 128 / G tokens x G heads is the tile, row by row). The
+// rest (the ends of a key range, pages of fewer than 8 tokens, other groups) is copied by both warps, 64 rows each,
+// 16 bytes per lane, with zeros for the rows that are not seen.
 template <typename T, int D>
 struct PtLoader {
   using Cfg = PtCfg<D>;
@@ -154,37 +144,39 @@ struct PtLoader {
   const PagedParams& p;
   const CUtensorMap* kmap;
   const CUtensorMap* vmap;
+  const CUtensorMap* qmap;
   uint32_t base;
   int w, lane;
-  int item;                                              // K/V tiles requested so far
-  int rows;                                              // of them, copied row by row and not handed over yet
+  int item, qitem;                                       // K/V tiles and query tiles so far
+  int rows, goes;                                        // tiles copied by rows and not handed over yet; times the warps met
 
-  __device__ __forceinline__ PtLoader(const PagedParams& p_, const CUtensorMap* k_, const CUtensorMap* v_, uint32_t base_, int w_,
-                                      int lane_)
-      : p(p_), kmap(k_), vmap(v_), base(base_), w(w_), lane(lane_), item(0), rows(0) {}
+  __device__ __forceinline__ PtLoader(const PagedParams& p_, const CUtensorMap* k_, const CUtensorMap* v_, const CUtensorMap* q_,
+                                      uint32_t base_, int w_, int lane_)
+      : p(p_), kmap(k_), vmap(v_), qmap(q_), base(base_), w(w_), lane(lane_), item(0), qitem(0), rows(0), goes(0) {}
 
-  __device__ __forceinline__ void signal(uint32_t bar) {
+  __device__ __forceinline__ bool wait(uint32_t off, uint32_t parity) { return pt_wait(base + off, parity, base + Cfg::OFF_MISC + 4); }
+  __device__ __forceinline__ bool wait_empty() { return wait(Cfg::EMPTY + 8 * (item % Cfg::ST), ((item / Cfg::ST) & 1) ^ 1); }
+  __device__ __forceinline__ uint32_t stage() const { return base + Cfg::OFF_KV + (item % Cfg::ST) * Cfg::TILEB; }
+  __device__ __forceinline__ void signal(uint32_t off) {
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) pt_arrive(bar);
+    if (lane == 0) pt_arrive(base + off);
   }
-  __device__ __forceinline__ bool wait_empty() {
-    return pt_wait(base + Cfg::EMPTY + 8 * (item % Cfg::ST), ((item / Cfg::ST) & 1) ^ 1, base + Cfg::OFF_MISC + 4);
-  }
-  __device__ __forceinline__ uint32_t full() const { return base + Cfg::FULL + 8 * (item % Cfg::ST); }
-  __device__ __forceinline__ uint32_t stage() const { return base + Cfg::OFF_KV + (item % Cfg::ST) * Cfg::TILEB; }
-  __device__ __forceinline__ int page(const int32_t* table, int t) const {
-    const int pg = table[t >> p.shift];
-    return pg >= 0 && pg < p.num_pages ? pg : -1;
-  }
-  // the boxes of one key tile: `pg` is the page of this lane's box (of p.box rows)
-  __device__ __forceinline__ void load_boxes(const CUtensorMap* map, int h, int n, int pg) {
-    const uint32_t bar = full();
-    if (lane == 0)
+  // the arrivals of both warps, and the bytes of one operand tile
+  __device__ __forceinline__ void expect(uint32_t bar) {
+    if (lane == 0) {
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 1;" ::"r"(bar) : "memory");
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)Cfg::TILEB) : "memory");
+    }
     __syncwarp();
-    const int boxes = PT_KT / p.box;
-    if (lane < boxes) {
+  }
+  __device__ __forceinline__ bool whole(const PtPiece& pc, int kv, int n) const {
+    return p.box > 0 && n * PT_KT >= pc.u.lo && n * PT_KT + PT_KT <= kv && n * PT_KT < pc.u.hi;
+  }
+  __device__ __forceinline__ void load_boxes(const CUtensorMap* map, int h, int n, int pg) {
+    const uint32_t bar = base + Cfg::FULL + 8 * (item % Cfg::ST);
+    expect(bar);
+    if (lane < PT_KT / p.box) {
       const int row = (n * PT_KT + lane * p.box) & ((1 << p.shift) - 1);
 #pragma unroll
       for (int half = 0; half < Cfg::NH; ++half)
@@ -195,121 +187,146 @@ struct PtLoader {
             : "memory");
     }
   }
-  __device__ __forceinline__ void load_rows(const T* pool, int64_t sp, int64_t st, int n, int pg) {
+  __device__ __forceinline__ void load_rows(const T* pool, int64_t sp, int64_t st, int n, int pg0, int pg1) {
     const int c = lane % CPR, mask = (1 << p.shift) - 1;
     const uint32_t col = stage() + (c >> 3) * PT_HALF;
 #pragma unroll 4
-    for (int j = 0; j < 32 / RPI; ++j) {
-      const int row = lane / CPR + j * RPI, ra = 32 * w + row;
-      const int g = __shfl_sync(0xffffffffu, pg, row);
+    for (int j = 0; j < 64 / RPI; ++j) {
+      const int row = lane / CPR + j * RPI, ra = 64 * w + row;
+      const int g = __shfl_sync(0xffffffffu, j < 32 / RPI ? pg0 : pg1, row & 31);
       const bool ok = g >= 0;
       const int64_t at = ok ? (int64_t)g * sp + (int64_t)((n * PT_KT + ra) & mask) * st + c * 8 : 0;
       cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), pool + at, ok);
     }
     cp_async_commit();
   }
-  __device__ __forceinline__ uint32_t qslot(int qitem) const { return qitem % Cfg::QS; }
-  // requests the query rows of row tile tl; qitem counts the tiles
-  __device__ __forceinline__ bool load_query(const PagedPlace& at, const PagedRequest& r, int tl, int qitem) {
-    const uint32_t slot = qslot(qitem);
-    const int total = r.q * p.G;
-    if (!pt_wait(base + Cfg::Q_EMPTY + 8 * slot, ((qitem / Cfg::QS) & 1) ^ 1, base + Cfg::OFF_MISC + 4)) return false;
-    const int flat = at.tile * PT_ROWS + tl * 128 + 32 * w + lane;
-    int64_t off = -1;
-    if (flat < total) {
-      const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
-      off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
-    }
-    const int c = lane % CPR;
-    const uint32_t col = base + Cfg::OFF_Q + slot * Cfg::TILEB + (c >> 3) * PT_HALF;
-#pragma unroll 4
-    for (int j = 0; j < 32 / RPI; ++j) {
-      const int row = lane / CPR + j * RPI, ra = 32 * w + row;
-      const int64_t o = __shfl_sync(0xffffffffu, off, row);
-      const bool ok = o >= 0;
-      cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), reinterpret_cast<const T*>(p.q) + (ok ? o + c * 8 : 0), ok);
-    }
-    cp_async_commit();
-    return true;
-  }
-  // Every row of the tile holds a token that the unit or a later token of the request sees: it may be copied as it is.
-  __device__ __forceinline__ bool whole(const PtPiece& pc, int kvlen, int n) const {
-    return n * PT_KT >= pc.u.lo && n * PT_KT + PT_KT <= kvlen && n * PT_KT < pc.u.hi;
-  }
-  __device__ __forceinline__ bool load_tile(const PtPiece& pc, int kvlen, int n, int h, const int32_t* table, int pg, bool boxes) {
-    if (boxes && __all_sync(0xffffffffu, pg >= 0 || lane >= PT_KT / p.box) && whole(pc, kvlen, n)) {
+  // requests the K and V rows of key tile n; `pg`: the page of this lane's box when the tile is whole
+  __device__ __forceinline__ bool load_tile(const PtPiece& pc, int kv, int n, int h, const int32_t* table, int pg) {
+    if (whole(pc, kv, n)) {
+      if (w == 0) {
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {
-        if (!wait_empty()) return false;
-        if (w == 0) load_boxes(kv == 0 ? kmap : vmap, h, n, pg);
-        else if (lane == 0) pt_arrive(full());
-        ++item;
+        for (int i = 0; i < 2; ++i, ++item) {
+          if (!wait_empty()) return false;
+          load_boxes(i == 0 ? kmap : vmap, h, n, pg);
+        }
+      } else {
+        item += 2;
       }
       return true;
     }
-    const int t = n * PT_KT + 32 * w + lane;
-    int mine = -1;
-    if (t >= pc.u.lo && t < pc.u.hi) {
-      mine = page(table, t);
-      if (mine < 0) atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+    // Both warps meet here: the second has not waited for the stages of the tiles in between, and a barrier's phases
+    // tell apart only neighbouring uses.
+    if (lane == 0) pt_arrive(base + Cfg::GO);
+    if (!wait(Cfg::GO, goes & 1)) return false;
+    ++goes;
+    int mine[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = n * PT_KT + 64 * w + 32 * i + lane;
+      mine[i] = -1;
+      if (t >= pc.u.lo && t < pc.u.hi) {
+        mine[i] = table[t >> p.shift];
+        if (mine[i] < 0 || mine[i] >= p.num_pages) {
+          atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+          mine[i] = -1;
+        }
+      }
     }
 #pragma unroll 1
-    for (int kv = 0; kv < 2; ++kv) {
+    for (int i = 0; i < 2; ++i, ++item, ++rows) {
       if (!wait_empty()) return false;
-      if (kv == 0) load_rows(reinterpret_cast<const T*>(p.key) + (int64_t)h * p.k_sh, p.k_sp, p.k_st, n, mine);
-      else load_rows(reinterpret_cast<const T*>(p.value) + (int64_t)h * p.v_sh, p.v_sp, p.v_st, n, mine);
-      ++item;
-      ++rows;
+      if (i == 0) load_rows(reinterpret_cast<const T*>(p.key) + (int64_t)h * p.k_sh, p.k_sp, p.k_st, n, mine[0], mine[1]);
+      else load_rows(reinterpret_cast<const T*>(p.value) + (int64_t)h * p.v_sh, p.v_sp, p.v_st, n, mine[0], mine[1]);
     }
     return true;
   }
-  // hands over what was copied row by row: `queries` row tiles from qitem on, requested before the last tile's rows
-  __device__ __forceinline__ void finish(int queries, int qitem) {
-    if (queries > 0) {
-      if (rows > 0) cp_async_wait<2>();
-      else cp_async_wait<0>();
-      for (int i = 0; i < queries; ++i) signal(base + Cfg::Q_FULL + 8 * qslot(qitem + i));
+  // requests the unit's query rows, `tiles` row tiles
+  __device__ __forceinline__ bool load_query(const PagedPlace& at, const PagedRequest& r, int tiles) {
+    const int total = r.q * p.G;
+    for (int tl = 0; tl < tiles; ++tl) {
+      const int slot = (qitem + tl) % Cfg::QS, f0 = at.tile * PT_ROWS + tl * 128;
+      const uint32_t dst = base + Cfg::OFF_Q + slot * Cfg::TILEB;
+      if (p.qbox > 0 && w > 0) continue;
+      if (!wait(Cfg::Q_EMPTY + 8 * slot, (((qitem + tl) / Cfg::QS) & 1) ^ 1)) return false;
+      if (p.qbox > 0) {
+        const uint32_t bar = base + Cfg::Q_FULL + 8 * slot;
+        expect(bar);
+        if (lane < Cfg::NH)
+          asm volatile(
+              "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+              ::"r"(dst + lane * PT_HALF), "l"(reinterpret_cast<uint64_t>(qmap)), "r"(bar), "r"(lane * 64), "r"(at.h * p.G),
+              "r"(r.first + f0 / p.G)
+              : "memory");
+        continue;
+      }
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int r0 = 64 * w + 32 * half, flat = f0 + r0 + lane;
+        int64_t off = -1;
+        if (flat < total) {
+          const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
+          off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
+        }
+        const int c = lane % CPR;
+        const uint32_t col = dst + (c >> 3) * PT_HALF;
+#pragma unroll 4
+        for (int j = 0; j < 32 / RPI; ++j) {
+          const int row = lane / CPR + j * RPI, ra = r0 + row;
+          const int64_t o = __shfl_sync(0xffffffffu, off, row);
+          const bool ok = o >= 0;
+          cp_async_16_or_zero(col + ra * 128 + (((c & 7) ^ (ra & 7)) << 4), reinterpret_cast<const T*>(p.q) + (ok ? o + c * 8 : 0), ok);
+        }
+      }
     }
+    if (p.qbox == 0) cp_async_commit();
+    return true;
+  }
+  // hands over what was copied by rows: the query tiles, when they were, and the K and V rows of the last tile
+  __device__ __forceinline__ void finish(int queries) {
+    if (p.qbox > 0) queries = 0;
+    if (queries == 0 && rows == 0) return;
+    cp_async_wait<0>();
+    for (int i = 0; i < queries; ++i) signal(Cfg::Q_FULL + 8 * ((qitem + i) % Cfg::QS));
     if (rows > 0) {
-      cp_async_wait<1>();
-      signal(base + Cfg::FULL + 8 * ((item - 2) % Cfg::ST));
-      cp_async_wait<0>();
-      signal(base + Cfg::FULL + 8 * ((item - 1) % Cfg::ST));
+      signal(Cfg::FULL + 8 * ((item - 2) % Cfg::ST));
+      signal(Cfg::FULL + 8 * ((item - 1) % Cfg::ST));
       rows = 0;
     }
   }
   __device__ __forceinline__ void run(PagedPlace at, PagedRequest r, long long left) {
-    int qitem = 0;
-    const bool tma = p.box > 0;
     bool ok = true;
     while (ok) {
       PtPiece pc;
       pc.set(p, at, r, left);
       const int32_t* table = p.table + (int64_t)at.b * p.table_st;
-      auto box_page = [&](int n) -> int {                // the page of this lane's box of a tile seen whole
-        if (!tma || n >= pc.n1 || !whole(pc, r.kv, n) || lane >= PT_KT / p.box) return -1;
-        return page(table, n * PT_KT + lane * p.box);
+      auto box_page = [&](int n) -> int {                // the page of this lane's box of a whole tile
+        if (w > 0 || n >= pc.n1 || !whole(pc, r.kv, n) || lane >= PT_KT / p.box) return 0;
+        const int pg = table[(n * PT_KT + lane * p.box) >> p.shift];
+        if (pg < 0 || pg >= p.num_pages) {
+          atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+          return p.num_pages;
+        }
+        return pg;
       };
       int pg = box_page(pc.n0);
       // The unit's query and first keys are requested together. With two query slots (D = 128) the query has to wait
       // for the last scores of the unit before this one; the first keys go ahead of it.
       const int queries = at.tile * PT_ROWS + 128 < r.q * p.G ? 2 : 1;
       const bool early = Cfg::QS == 4 || qitem == 0;
-      auto request = [&]() { return load_query(at, r, 0, qitem) && (queries < 2 || load_query(at, r, 1, qitem + 1)); };
-      ok = !early || request();
+      ok = !early || load_query(at, r, queries);
       for (int n = pc.n0; n < pc.n1 && ok; ++n) {
         const int next = box_page(n + 1);
-        ok = load_tile(pc, r.kv, n, at.h, table, pg, tma);
+        ok = load_tile(pc, r.kv, n, at.h, table, pg);
         if (!ok) break;
         if (n == pc.n0) {
-          finish(early ? queries : 0, qitem);
+          finish(early ? queries : 0);
           if (!early) {
-            ok = request();
-            if (ok) finish(queries, qitem);
+            ok = load_query(at, r, queries);
+            if (ok) finish(queries);
           }
-          qitem += queries;
+          if (ok) qitem += queries;
         } else {
-          finish(0, 0);
+          finish(0);
         }
         pg = next;
       }
@@ -318,6 +335,10 @@ struct PtLoader {
       if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
     }
     cp_async_wait<0>();
+    if (!ok && w == 0) {                                 // nothing of this block may land after it has left
+      for (int i = max(0, item - Cfg::ST); i < item; ++i) pt_wait(base + Cfg::FULL + 8 * (i % Cfg::ST), (i / Cfg::ST) & 1, base + Cfg::OFF_MISC + 8);
+      for (int i = max(0, qitem - Cfg::QS); i < qitem; ++i) pt_wait(base + Cfg::Q_FULL + 8 * (i % Cfg::QS), (i / Cfg::QS) & 1, base + Cfg::OFF_MISC + 8);
+    }
   }
 };
 
@@ -332,21 +353,26 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
   const uint32_t base = __shfl_sync(0xffffffffu, base_, 0), tmem = __shfl_sync(0xffffffffu, tmem_, 0);
   const uint32_t full = base + Cfg::FULL, empty = base + Cfg::EMPTY, s_full = base + Cfg::S_FULL, p_full = base + Cfg::P_FULL;
   const uint32_t dead = base + Cfg::OFF_MISC + 4;
-  const uint32_t elect = (threadIdx.x & 31) == 0 ? 1u : 0u;
   constexpr uint32_t id_s = pt_idesc<T>(PT_KT, false), id_o = pt_idesc<T>(D, true);
   uint32_t stage = 0, phase = 0;                         // of the next K/V tile
-  uint32_t qslot[2] = {0, 0}, qnext = 0, qphase = 0, p_use[2] = {0, 0};
+  uint32_t qslot[2] = {0, 0}, qaddr[2] = {0, 0}, qnext = 0, qphase = 0, p_use[2] = {0, 0};
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, pt_wait(bar, parity, dead)); };
-  auto commit = [&](uint32_t bar) { pt_commit(bar, elect); };
+  auto commit = [&](uint32_t bar) {
+    if (pt_elect()) pt_commit(bar);
+    __syncwarp();
+  };
   auto step = [&]() { if (++stage == Cfg::ST) { stage = 0; phase ^= 1; } };
   auto scores = [&](int w, uint32_t st) {
-    const uint32_t q = (base + Cfg::OFF_Q + qslot[w] * Cfg::TILEB) >> 4, k = (base + Cfg::OFF_KV + st * Cfg::TILEB) >> 4;
+    const uint32_t q = qaddr[w], k = (base + Cfg::OFF_KV + st * Cfg::TILEB) >> 4;
+    if (pt_elect()) {
 #pragma unroll
-    for (int h = 0; h < Cfg::NH; ++h)
+      for (int h = 0; h < Cfg::NH; ++h)
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        pt_mma_ss(tmem + Cfg::TS + 128 * w, pt_desc(q + ((h * PT_HALF + s * 32) >> 4), 16), pt_desc(k + ((h * PT_HALF + s * 32) >> 4), 16),
-                  id_s, h + s > 0 ? 1u : 0u, elect);
+        for (int s = 0; s < 4; ++s)
+          pt_mma_ss(tmem + Cfg::TS + 128 * w, pt_desc(q + ((h * PT_HALF + s * 32) >> 4), 16), pt_desc(k + ((h * PT_HALF + s * 32) >> 4), 16),
+                    id_s, h + s > 0 ? 1u : 0u);
+    }
+    __syncwarp();
   };
   while (true) {
     PtPiece pc;
@@ -367,6 +393,7 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
       if (w < tiles) {
         ok = ok && wait(base + Cfg::Q_FULL + 8 * qnext, qphase);
         qslot[w] = qnext;
+        qaddr[w] = __shfl_sync(0xffffffffu, (base + Cfg::OFF_Q + qnext * Cfg::TILEB) >> 4, 0);
         if (++qnext == Cfg::QS) { qnext = 0; qphase ^= 1; }
       }
     if (!ok) break;
@@ -401,10 +428,13 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
             ok = ok && wait(p_full + 16 * half + 8 * w, p_use[w] & 1);
             if (ok) {
               tc_fence_after();
+              if (pt_elect()) {
 #pragma unroll
-              for (int j = 4 * half; j < 4 * half + 4; ++j)
-                pt_mma_ts(tmem + Cfg::TO + D * w, tmem + Cfg::TS + 128 * w + 8 * j, pt_desc(v + j * 128, PT_HALF), id_o,
-                          (n > na[w] || j > 0) ? 1u : 0u, elect);
+                for (int j = 4 * half; j < 4 * half + 4; ++j)
+                  pt_mma_ts(tmem + Cfg::TO + D * w, tmem + Cfg::TS + 128 * w + 8 * j, pt_desc(v + j * 128, PT_HALF), id_o,
+                          (n > na[w] || j > 0) ? 1u : 0u);
+              }
+              __syncwarp();
             }
           }
           ++p_use[w];
@@ -430,7 +460,8 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
 
 // ---- softmax of one row tile: 4 warps, one row per thread ------------------------------------------------
 template <typename T, int D, bool MOD>
-__device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, uint32_t tmem, int w, int tid, PagedPlace at, PagedRequest r, long long left) {
+__device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, uint32_t tmem, int w, int tid, PagedPlace at, PagedRequest r, long long left, long long x,
+                                           long long per) {
   using Cfg = PtCfg<D>;
   const uint32_t s_full = base + Cfg::S_FULL + 8 * w, p_full = base + Cfg::P_FULL + 8 * w, dead = base + Cfg::OFF_MISC + 4;
   const int warp = tid >> 5, lane = tid & 31;
@@ -496,12 +527,14 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
           largest(v[0]);
         }
       } else {
-        TcLd<32>::ld(ts, v[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          TcLd<32>::wait(v[c & 1]);
-          if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
-          largest(v[c & 1]);
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          TcLd<32>::ld(ts + 32 * c, v[0]);
+          TcLd<32>::ld(ts + 32 * c + 32, v[1]);
+          TcLd<32>::wait(v[0]);
+          TcLd<32>::wait(v[1]);
+          largest(v[0]);
+          largest(v[1]);
         }
       }
       if (MOD || edge) tc_wait_st();
@@ -514,7 +547,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
         m = mn;
         l *= a;
         if (n > na) {                                    // the product before this one is complete: it was issued before these scores
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             TcLd<32>::ld(to + 32 * c, o);
@@ -523,46 +556,34 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
             tc_st32(to + 32 * c, o);
           }
-          TcLd<32>::ld(ts, v[0]);
         }
       }
       const float ms = m == -INFINITY ? 0.0f : m;
-      // Pass 2: weights, two at a time. PT_POLY pairs of every four come from a polynomial on the FMA pipe instead of the exponential unit,
-      // where the tile sees no mask: 16 exponentials per SM and cycle are as slow as both products together.
+      // Pass 2: weights, two at a time.
       const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
       uint64_t sum[2] = {0, 0};
-      auto weights = [&](auto poly) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-          TcLd<32>::wait(v[c & 1]);
-          if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+        TcLd<32>::wait(v[c & 1]);
+        if (c < 3) TcLd<32>::ld(ts + 32 * (c + 1), v[(c + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t y = fma2(pack2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), scale2, ms2);
-            float a, b;
-            uint64_t x;
-            if (decltype(poly)::value && i % 4 < PT_POLY) {
-              x = ex2_poly2(y);
-            } else {
-              unpack2(y, a, b);
-              x = pack2(ex2(a), ex2(b));
-            }
-            sum[i & 1] = add2(sum[i & 1], x);
-            unpack2(x, a, b);
-            pk[i] = Half2Of<T>::pack(a, b);
-          }
-          tc_st16(ts + 16 * c, pk);
-          if (c & 1) {                                   // half of the keys: the second product may begin
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) pt_arrive(p_full + 16 * (c >> 1));
-          }
+        for (int i = 0; i < 16; ++i) {
+          float a, b;
+          unpack2(fma2(pack2(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), scale2, ms2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum[i & 1] = add2(sum[i & 1], pack2(a, b));
+          pk[i] = Half2Of<T>::pack(a, b);
         }
-      };
-      if (edge) weights(std::false_type());
-      else weights(std::true_type());
+        tc_st16(ts + 16 * c, pk);
+        if (c & 1) {                                     // half of the keys: the second product may begin
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) pt_arrive(p_full + 16 * (c >> 1));
+        }
+      }
       float s0, s1;
       unpack2(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
@@ -579,7 +600,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
     const int slot = 2 * blockIdx.x + (pc.begins ? 1 : 0);
     const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
     const int64_t row = (int64_t)(r.first + token) * p.Hq + head;
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t o[32];
       if (some) {
@@ -610,8 +631,11 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       if (!whole) p.ws_ml[(int64_t)slot * PT_ROWS + w * 128 + tid] = make_float2(m, l);
       else if (p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * PA_LN2;
     }
-    if (!whole && w == 0 && tid == 0)
-      p.ws_desc[slot] = pc.begins ? make_int4(1, at.b, at.h, at.tile) : make_int4(1, pc.ends ? 1 : 0, 0, 0);
+    if (pc.begins && !pc.ends && w == 0 && tid == 0) {
+      p.ws_desc[2 * blockIdx.x] = make_int4(paged_pieces(per, x, pc.u.n, PT_SNAP, blockIdx.x), at.h, at.tile, 0);
+      p.ws_desc[2 * blockIdx.x + 1] = make_int4(r.first, r.q, 0, 0);
+    }
+    x += pc.n1 - pc.n0;
     tc_fence_before();                                   // the next unit's product overwrites the output once its weights are signalled
     left -= pc.n1 - pc.n0;
     if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) return;
@@ -633,7 +657,8 @@ __device__ __forceinline__ void pt_own(PagedPlace& at, PagedRequest& r, long lon
 // product is complete. Rows of K and V outside what the unit sees are zero-filled, not read.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
-    paged_chunk_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    paged_chunk_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const __grid_constant__ CUtensorMap qmap) {
   using Cfg = PtCfg<D>;
   extern __shared__ uint8_t pt_raw[];
   const uint32_t raw = smem_u32(pt_raw);
@@ -644,24 +669,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in all lanes, and known to be
   pdl_launch_dependents();
 
-  PagedPlace at;
-  long long left;
-  paged_span<PT_ROWS, PT_KT, PT_THREADS>(p, reinterpret_cast<int*>(smem + Cfg::OFF_KV), at, left, 2);
-  if (tid < 2) p.ws_desc[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
-  if (left <= 0) return;
+  const PagedSpan span = paged_span<PT_ROWS, PT_KT, PT_THREADS>(p, reinterpret_cast<int*>(smem + Cfg::OFF_KV), PT_SNAP, PT_LEAST);
+  if (tid == 0) p.ws_desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (span.left <= 0) return;
+  PagedPlace at = span.at;
+  long long left = span.left;
   if (warp == 0) {
     tc_alloc(s_tmem, 512);
     tc_relinquish();
   }
   if (tid == 32) {
-    s_tmem[1] = 0;
+    s_tmem[1] = s_tmem[2] = 0;
     auto bar = [&](int off) { return reinterpret_cast<uint64_t*>(smem + off); };
     for (int i = 0; i < Cfg::QS; ++i) {
-      mbar_init(bar(Cfg::Q_FULL + 8 * i), 4);
+      mbar_init(bar(Cfg::Q_FULL + 8 * i), 2);
       mbar_init(bar(Cfg::Q_EMPTY + 8 * i), 1);
     }
     for (int i = 0; i < Cfg::ST; ++i) {
-      mbar_init(bar(Cfg::FULL + 8 * i), 4);
+      mbar_init(bar(Cfg::FULL + 8 * i), 2);
       mbar_init(bar(Cfg::EMPTY + 8 * i), 1);
     }
     for (int w = 0; w < 2; ++w) {
@@ -670,6 +695,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       mbar_init(bar(Cfg::P_FULL + 16 + 8 * w), 4);
     }
     mbar_init(bar(Cfg::DONE), 1);
+    mbar_init(bar(Cfg::GO), 2);
     fence_mbar_init();
   }
   PagedRequest r = paged_request(p, at.b);
@@ -678,20 +704,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  // registers: 128 x 512 at launch = 192 x 256 + 64 x 128 + 64 x 128
+  // registers: 168 x 384 at launch = 208 x 256 + 88 x 128
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     pt_own(at, r, left);
-    pt_softmax<T, D, MOD>(p, base, tmem, warp >> 2, tid & 127, at, r, left);
-  } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    pt_own(at, r, left);
-    PtLoader<T, D> loader(p, &kmap, &vmap, base, warp - 8, lane);
-    loader.run(at, r, left);
+    pt_softmax<T, D, MOD>(p, base, tmem, warp >> 2, tid & 127, at, r, left, span.x, span.per);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (warp == 12) {
-      pt_own(at, r, left);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    pt_own(at, r, left);
+    if (warp < 10) {
+      PtLoader<T, D> loader(p, &kmap, &vmap, &qmap, base, warp - 8, lane);
+      loader.run(at, r, left);
+    } else if (warp == 10) {
       pt_issue<T, D>(p, base, tmem, at, r, left);
     }
   }

@@ -41,12 +41,14 @@ struct PagedParams {
   float2* ws_ml;                                     // [2*grid][ROWS] (m, l)
   int4* ws_desc;                                     // [2*grid]: see PieceDesc
   int grid;
+  int few_tiles;                                     // whether all key tiles can be counted in 31 bits
   int box;                                           // rows per TMA box of a pool, 0: no TMA
+  int qbox;                                          // tokens per TMA box of the query, 0: no TMA
 };
 
-// ws_desc[2c]: the piece that continues a unit begun by an earlier block: x = 1, y = 1 iff the unit ends in it.
-// ws_desc[2c+1]: the piece that begins a unit which a later block ends: x = 1, y = request, z = KV head, w = row tile.
-// x = 0: no such piece.
+// ws_desc[2c], ws_desc[2c+1]: the unit that span c begins and a later one ends: {pieces, KV head, row tile, 0} and the
+// request's {first row, new tokens, 0, 0}; pieces == 0 when there is none. The first piece lies at slot 2c+1, the
+// pieces of the spans after it at slots 2(c+1), 2(c+2), ...
 
 struct PagedRequest {
   int first, q, kv, pre;      // first row of the packed query, new tokens, keys, prefix; position of token i: kv - q + i
@@ -92,48 +94,156 @@ __device__ __forceinline__ int paged_row_tiles(const PagedRequest& r, int G) {
 }
 
 struct PagedPlace { int b, h, tile, k; };            // a key tile: request, KV head, row tile, key tile of the unit
+struct PagedSpan {
+  PagedPlace at;                                       // the block's first key tile, at position x of all
+  long long x, left, per;                              // how many it has; the length of a span before its ends are moved
+};
 
-// Cuts the work. Called by every thread of the block; s_sum: B words of shared memory, free again afterwards.
-// Returns the block's first key tile and how many it has.
-template <int ROWS, int KT, int THREADS>
-__device__ __forceinline__ void paged_span(const PagedParams& p, int* s_sum, PagedPlace& place, long long& count, int snap) {
-  __shared__ long long s_total;
-  __shared__ PagedPlace s_place[2];
-  __shared__ long long s_pos[2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int WARPS = THREADS / 32;
-  // key tiles of one KV head of every request
-  for (int b0 = warp * 32; b0 < p.B; b0 += WARPS * 32) {
-    const int b = b0 + lane;
-    PagedRequest r = {0, 0, 0, 0};
-    int tiles = 0, sum = 0;
-    if (b < p.B) {
-      r = paged_request(p, b);
-      tiles = paged_row_tiles<ROWS>(r, p.G);
-      if (tiles <= 4)
-        for (int t = 0; t < tiles; ++t) {
-          PagedUnit<ROWS, KT> u;
-          u.set(r, p.G, p.window, t);
-          sum += u.n;
-        }
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);      // a 64-bit division takes a hundred instructions
+}
+
+// Key tiles of one KV head of the request of every lane (all lanes call).
+template <int ROWS, int KT>
+__device__ __forceinline__ int paged_lane_sum(const PagedParams& p, const PagedRequest& r, int lane) {
+  const int tiles = paged_row_tiles<ROWS>(r, p.G);
+  int sum = 0;
+  if (tiles <= 4)
+    for (int t = 0; t < tiles; ++t) {
+      PagedUnit<ROWS, KT> u;
+      u.set(r, p.G, p.window, t);
+      sum += u.n;
     }
-    unsigned big = __ballot_sync(0xffffffffu, tiles > 4);
-    while (big) {
-      const int src = __ffs(big) - 1;
-      big &= big - 1;
-      const PagedRequest rr = {__shfl_sync(0xffffffffu, r.first, src), __shfl_sync(0xffffffffu, r.q, src),
-                               __shfl_sync(0xffffffffu, r.kv, src), __shfl_sync(0xffffffffu, r.pre, src)};
-      const int nt = __shfl_sync(0xffffffffu, tiles, src);
-      int part = 0;
-      for (int t = lane; t < nt; t += 32) {
-        PagedUnit<ROWS, KT> u;
-        u.set(rr, p.G, p.window, t);
-        part += u.n;
+  unsigned big = __ballot_sync(0xffffffffu, tiles > 4);
+  while (big) {
+    const int src = __ffs(big) - 1;
+    big &= big - 1;
+    const PagedRequest rr = {0, __shfl_sync(0xffffffffu, r.q, src), __shfl_sync(0xffffffffu, r.kv, src), __shfl_sync(0xffffffffu, r.pre, src)};
+    const int nt = __shfl_sync(0xffffffffu, tiles, src);
+    int part = 0;
+    for (int t = lane; t < nt; t += 32) {
+      PagedUnit<ROWS, KT> u;
+      u.set(rr, p.G, p.window, t);
+      part += u.n;
+    }
+    part = __reduce_add_sync(0xffffffffu, part);
+    if (lane == src) sum = part;
+  }
+  return sum;
+}
+
+// The row tile of a request in which key tile k of one KV head lies; k becomes its place in the unit, n the unit's length.
+template <int ROWS, int KT>
+__device__ __forceinline__ int paged_find_tile(const PagedParams& p, const PagedRequest& r, int nt, int& k, int& n, int lane) {
+  int run = 0;
+  for (int t0 = 0; t0 < nt; t0 += 32) {
+    PagedUnit<ROWS, KT> u;
+    u.n = 0;
+    if (t0 + lane < nt) u.set(r, p.G, p.window, t0 + lane);
+    int inc = u.n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, run + inc > k);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      n = __shfl_sync(0xffffffffu, u.n, l);
+      k -= run + __shfl_sync(0xffffffffu, inc - u.n, l);
+      return t0 + l;
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return nt;
+}
+
+// Moves a cut (at.k key tiles into a unit of n, position x) to the unit's edge when it lies within `snap` of one. True
+// when that is the end of the request's last unit: the place is then the next request that has rows.
+template <typename I>
+__device__ __forceinline__ bool paged_snap(const PagedParams& p, PagedPlace& at, I& x, int n, int nt, int snap) {
+  if (at.k == 0) return false;
+  if (at.k <= snap) {
+    x -= at.k;
+    at.k = 0;
+  } else if (n - at.k <= snap) {
+    x += n - at.k;
+    at.k = 0;
+    if (++at.tile == nt) {
+      at.tile = 0;
+      if (++at.h == p.Hkv) {
+        at.h = 0;
+        return true;
       }
-      part = __reduce_add_sync(0xffffffffu, part);
-      if (lane == src) sum = part;
     }
-    if (b < p.B) s_sum[b] = sum;
+  }
+  return false;
+}
+
+// Cuts the work. Called by every thread of the block; s_sum: B words of shared memory, free again afterwards. With up
+// to 32 requests every warp finds the span by itself, one request per lane, after one round trip to memory and with
+// little code: what a block does before its first load costs a short call more than all the rest (this part took 9500
+// cycles when one routine served all cases).
+template <int ROWS, int KT, int THREADS>
+__device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int* s_sum, int snap, int least) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PagedSpan out;
+  out.at = {p.B, 0, 0, 0};
+  if (p.B <= 32 && p.few_tiles) {
+    PagedRequest mine = {0, 0, 0, 0};
+    if (lane < p.B) mine = paged_request(p, lane);
+    const int tiles = paged_row_tiles<ROWS>(mine, p.G);
+    int sum;
+    if (__any_sync(0xffffffffu, tiles > 1)) {
+      sum = paged_lane_sum<ROWS, KT>(p, mine, lane);
+    } else {
+      PagedUnit<ROWS, KT> u;
+      u.set(mine, p.G, p.window, 0);
+      sum = tiles > 0 ? u.n : 0;
+    }
+    int inc = sum * p.Hkv;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    const int total = __shfl_sync(0xffffffffu, inc, 31);
+    const int per = max(least, (int)(((unsigned)total + gridDim.x - 1) / gridDim.x));
+    int x = 0, end = 0;
+#pragma unroll 1
+    for (int i = 1; i >= 0; --i) {                       // the end, then the beginning
+      const long long want = (long long)per * (blockIdx.x + i);
+      x = want < total ? (int)want : total;
+      if (x < total) {
+        const int b = __ffs(__ballot_sync(0xffffffffu, inc > x)) - 1;
+        const int per_head = __shfl_sync(0xffffffffu, sum, b), rem = x - __shfl_sync(0xffffffffu, inc - sum * p.Hkv, b);
+        const int nt = __shfl_sync(0xffffffffu, tiles, b);
+        int n = per_head;
+        out.at = {b, rem / per_head, 0, rem % per_head};
+        if (nt > 1) {
+          const PagedRequest r = {0, __shfl_sync(0xffffffffu, mine.q, b), __shfl_sync(0xffffffffu, mine.kv, b), __shfl_sync(0xffffffffu, mine.pre, b)};
+          out.at.tile = paged_find_tile<ROWS, KT>(p, r, nt, out.at.k, n, lane);
+        }
+        if (paged_snap(p, out.at, x, n, nt, snap)) {
+          const unsigned rows = __ballot_sync(0xffffffffu, sum > 0) & (0xfffffffeu << b);
+          out.at.b = rows ? __ffs(rows) - 1 : p.B;
+        }
+      }
+      if (i == 1) end = x;
+    }
+    out.x = x;
+    out.left = end - x;
+    out.per = per;
+    return out;
+  }
+  __shared__ long long s_total;
+  __shared__ PagedPlace s_place;
+  __shared__ long long s_pos[2];
+  for (int b0 = warp * 32; b0 < p.B; b0 += THREADS) {
+    PagedRequest r = {0, 0, 0, 0};
+    if (b0 + lane < p.B) r = paged_request(p, b0 + lane);
+    const int sum = paged_lane_sum<ROWS, KT>(p, r, lane);
+    if (b0 + lane < p.B) s_sum[b0 + lane] = sum;
   }
   __syncthreads();
   if (warp == 0) {
@@ -144,18 +254,16 @@ __device__ __forceinline__ void paged_span(const PagedParams& p, int* s_sum, Pag
     if (lane == 0) s_total = t * p.Hkv;
   }
   __syncthreads();
+  const long long total = s_total;
+  out.per = max((long long)least, paged_div(total + gridDim.x - 1, gridDim.x));
   if (warp < 2) {
     // warp 0 finds the first tile of this block's span, warp 1 that of the next block's
-    const long long total = s_total;
-    const long long per = (total + gridDim.x - 1) / gridDim.x;
-    long long x = per * (blockIdx.x + warp);
+    long long x = min(total, out.per * (blockIdx.x + warp));
     PagedPlace at = {p.B, 0, 0, 0};
-    if (x >= total) {
-      x = total;
-    } else {
+    if (x < total) {
       long long base = 0;
       int b = -1;
-      for (int b0 = 0; b0 < p.B && b < 0; b0 += 32) {
+      for (int b0 = 0; b < 0; b0 += 32) {
         const long long s = b0 + lane < p.B ? (long long)s_sum[b0 + lane] * p.Hkv : 0;
         long long inc = s;
 #pragma unroll
@@ -173,62 +281,32 @@ __device__ __forceinline__ void paged_span(const PagedParams& p, int* s_sum, Pag
         }
       }
       const PagedRequest r = paged_request(p, b);
-      const int nt = paged_row_tiles<ROWS>(r, p.G);
-      long long rem = x - base;
-      const int per_head = s_sum[b];
-      int h = (int)(rem / per_head);
-      int k = (int)(rem - (long long)h * per_head);
-      int tile = 0, n = 1;
-      int run = 0;
-      bool found = false;
-      for (int t0 = 0; t0 < nt && !found; t0 += 32) {
-        PagedUnit<ROWS, KT> u;
-        u.n = 0;
-        if (t0 + lane < nt) u.set(r, p.G, p.window, t0 + lane);
-        int inc = u.n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int o = __shfl_up_sync(0xffffffffu, inc, d);
-          if (lane >= d) inc += o;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run + inc > k);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          tile = t0 + l;
-          n = __shfl_sync(0xffffffffu, u.n, l);
-          k -= run + __shfl_sync(0xffffffffu, inc - u.n, l);
-          found = true;
-        } else {
-          run += __shfl_sync(0xffffffffu, inc, 31);
-        }
-      }
-      if (k > 0) {
-        if (k <= snap) {
-          x -= k;
-          k = 0;
-        } else if (n - k <= snap) {                  // the next unit; its place is found by walking on
-          x += n - k;
-          k = 0;
-          if (++tile == nt) {
-            tile = 0;
-            if (++h == p.Hkv) {
-              h = 0;
-              do { ++b; } while (b < p.B && s_sum[b] == 0);
-            }
-          }
-        }
-      }
-      at = {b, h, tile, k};
+      const int nt = paged_row_tiles<ROWS>(r, p.G), per_head = s_sum[b];
+      const long long rem = x - base;
+      at = {b, (int)paged_div(rem, per_head), 0, 0};
+      at.k = (int)(rem - (long long)at.h * per_head);
+      int n = per_head;
+      at.tile = paged_find_tile<ROWS, KT>(p, r, nt, at.k, n, lane);
+      if (paged_snap(p, at, x, n, nt, snap))
+        do { ++at.b; } while (at.b < p.B && s_sum[at.b] == 0);
     }
     if (lane == 0) {
-      s_place[warp] = at;
+      if (warp == 0) s_place = at;
       s_pos[warp] = x;
     }
   }
   __syncthreads();
-  place = s_place[0];
-  count = s_pos[1] - s_pos[0];
+  out.at = s_place;
+  out.x = s_pos[0];
+  out.left = s_pos[1] - s_pos[0];
   __syncthreads();
+  return out;
+}
+
+// How many pieces the unit [x - k, x - k + n) has whose first piece span c holds, when span c ends before the unit does:
+// the cuts behind c that fall inside it, none within `snap` of its edges.
+__device__ __forceinline__ int paged_pieces(long long per, long long begin, int n, int snap, int c) {
+  return (int)(paged_div(begin + n - snap - 1, per) - c) + 1;
 }
 
 // The unit after (b, h, tile): next row tile, next KV head, next request that has rows. False when there is none.
@@ -327,20 +405,21 @@ __device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, flo
     for (int i = 0; i < N; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), scale2), x[i], x[i + 1]);
   }
   if (p.slopes) {
-    const uint64_t d2 = pack2((float)d0, (float)d0);
-    if (__all_sync(0xffffffffu, d0 + N <= 1)) {          // no key behind its query: |p - j| = p - j
-      const uint64_t s2 = pack2(slope_log2, slope_log2);
+    // distances are whole numbers below 2^24, exact in fp32: four running pairs instead of a constant for each
+    constexpr int R = N >= 8 ? 4 : N / 2;
+    const bool behind = __any_sync(0xffffffffu, d0 + N > 1);     // some key behind its query: |p - j| is not p - j
+    const uint64_t s2 = behind ? pack2(-slope_log2, -slope_log2) : pack2(slope_log2, slope_log2);
+    const uint64_t step = pack2((float)(2 * R), (float)(2 * R));
+    uint64_t d[R];
 #pragma unroll
-      for (int i = 0; i < N; i += 2)
-        unpack2(fma2(add2(d2, pack2((float)i, (float)(i + 1))), s2, pack2(x[i], x[i + 1])), x[i], x[i + 1]);
-    } else {
-      const uint64_t s2 = pack2(-slope_log2, -slope_log2);
+    for (int i = 0; i < R; ++i) d[i] = pack2((float)(d0 + 2 * i), (float)(d0 + 2 * i + 1));
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        float a, b;
-        unpack2(add2(d2, pack2((float)i, (float)(i + 1))), a, b);
-        unpack2(fma2(pack2(fabsf(a), fabsf(b)), s2, pack2(x[i], x[i + 1])), x[i], x[i + 1]);
-      }
+    for (int i = 0; i < N / 2; ++i) {
+      float a, b;
+      unpack2(d[i % R], a, b);
+      if (behind) { a = fabsf(a); b = fabsf(b); }
+      unpack2(fma2(pack2(a, b), s2, pack2(x[2 * i], x[2 * i + 1])), x[2 * i], x[2 * i + 1]);
+      if (i + R < N / 2) d[i % R] = add2(d[i % R], step);
     }
   }
 }
@@ -382,75 +461,62 @@ __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst_smem, const voi
 // Joins the pieces of the units that a cut divided: block (c, y) takes the unit that span c leaves unfinished,
 // rows y*RB ... of its tile, one warp per row:
 //     M = max m_s,  out = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
+// Bound by round trips to L2: the descriptor, then (m, l) of up to 32 pieces at once and the outputs beside them.
 constexpr int PM_WARPS = 4;
 template <typename T, int D, int ROWS, int RPW>
 __global__ void __launch_bounds__(PM_WARPS * 32) paged_merge_kernel(PagedParams p) {
-  __shared__ float s_w[PM_WARPS][512];
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  const int4 d = p.ws_desc[2 * c + 1];
-  if (d.x == 0) return;
-  const PagedRequest r = paged_request(p, d.y);
-  const int rows = min(ROWS, r.q * p.G - d.w * ROWS);
+  const int4 d = p.ws_desc[2 * c], e = p.ws_desc[2 * c + 1];
+  const int n = d.x;
+  if (n == 0) return;
+  const int rows = min(ROWS, e.y * p.G - d.z * ROWS);
   const int row0 = (blockIdx.y * PM_WARPS + warp) * RPW;
-  if (blockIdx.y * PM_WARPS * RPW >= rows) return;
-  // pieces: slot 2c+1, then 2(c+1), 2(c+2), ... up to the one that ends the unit
-  int last = c + 1;
-  while (true) {
-    const int k = last + lane;
-    const int4 e = k < p.grid ? p.ws_desc[2 * k] : make_int4(0, 1, 0, 0);
-    const unsigned stop = __ballot_sync(0xffffffffu, e.x == 0 || e.y != 0);
-    if (stop) {
-      last += __ffs(stop) - 1;
-      break;
-    }
-    last += 32;
-  }
-  const int n = min(last, p.grid - 1) - c + 1;
+  constexpr int E = D / 32;
+  auto slot = [&](int s) -> int64_t { return s == 0 ? 2 * c + 1 : 2 * (c + s); };
   for (int rr = row0; rr < min(row0 + RPW, rows); ++rr) {
-    float m = -INFINITY;
-    for (int s = lane; s < n; s += 32) m = fmaxf(m, p.ws_ml[(int64_t)(s == 0 ? 2 * c + 1 : 2 * (c + s)) * ROWS + rr].x);
+    float m = -INFINITY, l = 0.0f, acc[E];
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ms = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int s = lane; s < n; s += 32) {
-      const float2 ml = p.ws_ml[(int64_t)(s == 0 ? 2 * c + 1 : 2 * (c + s)) * ROWS + rr];
-      const float w = exp2f(ml.x - ms);
-      s_w[warp][s] = w;
-      l = fmaf(w, ml.y, l);
-    }
+    for (int i = 0; i < E; ++i) acc[i] = 0.0f;
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      const float2 ml = s0 + lane < n ? p.ws_ml[slot(s0 + lane) * ROWS + rr] : make_float2(-INFINITY, 0.0f);
+      float top = ml.x;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    __syncwarp();
-    constexpr int E = D / 32;
-    float acc[E];
+      for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.0f : mn;
+      const float old = exp2f(m - ms), w = exp2f(ml.x - ms);
+      float part = w * ml.y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float* o = p.ws_o + ((int64_t)(s == 0 ? 2 * c + 1 : 2 * (c + s)) * ROWS + rr) * D + lane * E;
-      const float w = s_w[warp][s];
-      if constexpr (E == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(o);
-        acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
-        acc[2] = fmaf(w, v.z, acc[2]); acc[3] = fmaf(w, v.w, acc[3]);
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(o);
-        acc[0] = fmaf(w, v.x, acc[0]); acc[1] = fmaf(w, v.y, acc[1]);
+      for (int o = 16; o >= 1; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      l = fmaf(l, old, part);
+      m = mn;
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] *= old;
+      const int k = min(32, n - s0);
+#pragma unroll 8
+      for (int s = 0; s < k; ++s) {
+        const float* o = p.ws_o + (slot(s0 + s) * ROWS + rr) * D + lane * E;
+        const float f = __shfl_sync(0xffffffffu, w, s);
+        if constexpr (E == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(o);
+          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
+          acc[2] = fmaf(f, v.z, acc[2]); acc[3] = fmaf(f, v.w, acc[3]);
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(o);
+          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
+        }
       }
     }
     const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);       // a NaN stays one
-    const int flat = d.w * ROWS + rr, token = flat / p.G, head = d.z * p.G + (flat - token * p.G);
-    const int64_t at = (int64_t)(r.first + token) * p.Hq + head;
+    const int flat = d.z * ROWS + rr, token = flat / p.G, head = d.y * p.G + (flat - token * p.G);
+    const int64_t at = (int64_t)(e.x + token) * p.Hq + head;
     T* out = reinterpret_cast<T*>(p.out) + at * D + lane * E;
     if constexpr (E == 4) {
       *reinterpret_cast<uint2*>(out) = make_uint2(Half2Of<T>::pack(acc[0] * inv, acc[1] * inv), Half2Of<T>::pack(acc[2] * inv, acc[3] * inv));
     } else {
       *reinterpret_cast<uint32_t*>(out) = Half2Of<T>::pack(acc[0] * inv, acc[1] * inv);
     }
-    if (p.lse && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (ms + log2f(l)) * PA_LN2;
-    __syncwarp();
+    if (p.lse && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * PA_LN2;
   }
 }
 
