@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
 
   while (true) {
     PagedUnit<PR_ROWS, PR_KT> u;
-    u.set(r, p.G, p.window, at.tile);
+    u.set(p, r, at.tile);
     const int ntile = (int)min((long long)(u.n - at.k), span.left);
     const bool begins = at.k == 0, ends = at.k + ntile == u.n;
     const int rows = min(PR_ROWS, r.q * p.G - at.tile * PR_ROWS);
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
     for (int i = 0; i < 2; ++i) {
       const int row = g + 8 * i, flat = at.tile * PR_ROWS + row;
       const bool live = row < rows;
-      const int token = live ? flat / p.G : 0, head = at.h * p.G + (live ? flat - token * p.G : 0);
+      const int token = live ? paged_token(p, flat) : 0, head = at.h * p.G + (live ? flat - token * p.G : 0);
       const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh + 2 * t4;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
       slope[i] = MOD && p.slopes && live ? p.slopes[head] * PA_LOG2E : 0.0f;
     }
     // keys that every row of the unit sees need no mask
-    const int all_lo = paged_lo(r, p.window, (at.tile * PR_ROWS + rows - 1) / p.G);
-    const int all_hi = paged_hi(r, at.tile * PR_ROWS / p.G);
+    const int all_lo = paged_lo(r, p.window, paged_token(p, at.tile * PR_ROWS + rows - 1));
+    const int all_hi = paged_hi(r, paged_token(p, at.tile * PR_ROWS));
 
     auto page_of = [&](int tile) -> int {               // lanes 16..31 mirror lanes 0..15
       const int t = key0 + tile * PR_KT + (lane & 15);
@@ -172,25 +172,27 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
       const bool edge = t0 < all_lo || t0 + 16 > all_hi;
       float x[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if constexpr (MOD) {
-            x[n][2 * w] = c[n][2 * w];
-            x[n][2 * w + 1] = c[n][2 * w + 1];
-            paged_scores<2>(p, &x[n][2 * w], slope[w], t0 + 8 * n + 2 * t4 - pos[w]);
-          } else {
-            x[n][2 * w] = c[n][2 * w] * p.scale_log2;
-            x[n][2 * w + 1] = c[n][2 * w + 1] * p.scale_log2;
-          }
+        for (int e = 0; e < 4; ++e) x[n][e] = MOD ? c[n][e] : c[n][e] * p.scale_log2;
+      if constexpr (MOD) {
+        paged_scale<8>(p, &x[0][0]);
+        if (p.slopes) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[n][e] = fmaf(-slope[e >> 1], fabsf((float)(t0 + 8 * n + 2 * t4 + (e & 1) - pos[e >> 1])), x[n][e]);
         }
-        if (edge)
+      }
+      if (edge)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = t0 + 8 * n + 2 * t4 + (e & 1), w = e >> 1;
             if (t < lo[w] || t >= hi[w]) x[n][e] = -INFINITY;
           }
-      }
       float mx[2];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
       }
       if (begins && ends) {
         const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
-        const int flat = at.tile * PR_ROWS + row, token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
+        const int flat = at.tile * PR_ROWS + row, token = paged_token(p, flat), head = at.h * p.G + (flat - token * p.G);
         const int64_t to = (int64_t)(r.first + token) * p.Hq + head;
         uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + to * D + lane * E);
 #pragma unroll
@@ -462,6 +464,7 @@ extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb
   p.num_pages = a->num_pages;
   p.cu_q = a->cu_q; p.kv_len = a->kv_len; p.prefix = a->prefix_len; p.slopes = a->slopes;
   p.N = a->N; p.B = a->B; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv; p.window = a->window;
+  p.g_shift = (p.G & (p.G - 1)) == 0 ? log2_int(p.G) : -1;
   p.scale_log2 = a->scaling * PA_LOG2E;
   if (a->softcap > 0.0f) { p.cap_in = a->scaling / a->softcap; p.cap_log2 = a->softcap * PA_LOG2E; }
   p.out = a->out; p.lse = a->lse;

@@ -113,7 +113,7 @@ struct PtPiece {
   int n0, n1;
   bool begins, ends;
   __device__ __forceinline__ void set(const PagedParams& p, const PagedPlace& at, const PagedRequest& r, long long left) {
-    u.set(r, p.G, p.window, at.tile);
+    u.set(p, r, at.tile);
     n0 = u.t0 + at.k;
     n1 = n0 + (int)min((long long)(u.n - at.k), left);
     begins = at.k == 0;
@@ -124,7 +124,7 @@ struct PtPiece {
     na = nb = n0;
     const int f0 = at.tile * PT_ROWS + w * 128;
     if (f0 >= r.q * p.G) return;
-    const int lo = paged_lo(r, p.window, f0 / p.G), hi = paged_hi(r, min(r.q - 1, (f0 + 127) / p.G));
+    const int lo = paged_lo(r, p.window, paged_token(p, f0)), hi = paged_hi(r, min(r.q - 1, paged_token(p, f0 + 127)));
     if (hi <= lo) return;
     const int a = max(n0, lo / PT_KT), b = min(n1, (hi + PT_KT - 1) / PT_KT);
     if (a < b) { na = a; nb = b; }
@@ -264,7 +264,7 @@ struct PtLoader {
         const int r0 = 64 * w + 32 * half, flat = f0 + r0 + lane;
         int64_t off = -1;
         if (flat < total) {
-          const int token = flat / p.G, head = at.h * p.G + (flat - token * p.G);
+          const int token = paged_token(p, flat), head = at.h * p.G + (flat - token * p.G);
           off = (int64_t)(r.first + token) * p.q_st + (int64_t)head * p.q_sh;
         }
         const int c = lane % CPR;
@@ -475,13 +475,13 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
     pc.rows(p, at, r, w, na, nb);
     const int flat = at.tile * PT_ROWS + w * 128 + tid;
     const bool live = flat < r.q * p.G;
-    const int token = live ? flat / p.G : 0, head = at.h * p.G + (live ? flat - token * p.G : 0);
+    const int token = live ? paged_token(p, flat) : 0, head = at.h * p.G + (live ? flat - token * p.G : 0);
     const int pos = r.kv - r.q + token;
     const int lo = live ? paged_lo(r, p.window, token) : 0, hi = live ? max(lo, paged_hi(r, token)) : 0;
     const float slope = MOD && p.slopes && live ? p.slopes[head] * PA_LOG2E : 0.0f;
     // keys that every row of the tile sees need no mask
     const int f0 = at.tile * PT_ROWS + w * 128;
-    const int all_lo = paged_lo(r, p.window, min(r.q - 1, (f0 + 127) / p.G)), all_hi = paged_hi(r, f0 / p.G);
+    const int all_lo = paged_lo(r, p.window, min(r.q - 1, paged_token(p, f0 + 127))), all_hi = paged_hi(r, paged_token(p, f0));
     const bool any = f0 + 32 * warp < r.q * p.G;         // whether the warp has a row at all
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -500,7 +500,6 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       // tile twice costs less than holding its 128 scores, which leaves the other roles too few registers.
       const int t0 = n * PT_KT;
       const bool edge = t0 < all_lo || t0 + PT_KT > all_hi;
-      const uint32_t from = (uint32_t)(lo - t0), width = (uint32_t)(hi - lo);
       uint32_t v[2][32];
       float mx[2] = {-INFINITY, -INFINITY};
       auto largest = [&](const uint32_t* x) {
@@ -516,12 +515,17 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
         for (int c = 0; c < 4; ++c) {
           TcLd<32>::ld(ts + 32 * c, v[0]);
           TcLd<32>::wait(v[0]);
-          if constexpr (MOD) paged_scores<32>(p, reinterpret_cast<float*>(v[0]), slope, t0 + 32 * c - pos);
+          if constexpr (MOD) {
+            paged_scale<32>(p, reinterpret_cast<float*>(v[0]));
+            if (p.slopes) paged_bias<32>(reinterpret_cast<float*>(v[0]), slope, t0 + 32 * c - pos);
+          }
           if (edge) {
-            const uint32_t at0 = (uint32_t)(32 * c) - from;
+            const uint32_t seen = paged_seen(t0 + 32 * c, lo, hi);
+            if (__any_sync(0xffffffffu, seen != 0xffffffffu)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (at0 + i >= width) v[0][i] = 0xff800000u;
+              for (int i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) v[0][i] = 0xff800000u;
+            }
           }
           tc_st32(ts + 32 * c, v[0]);
           largest(v[0]);

@@ -33,6 +33,7 @@ struct PagedParams {
   const int32_t* prefix;                             // [B] or NULL
   const float* slopes;                               // [Hq] or NULL
   int N, B, Hq, Hkv, G, window;
+  int g_shift;                                       // log2(G), -1 when it is not a power of two
   float scale_log2;                                  // scaling * log2(e)
   float cap_in, cap_log2;                            // scaling / softcap, softcap * log2(e); cap_log2 == 0: none
   void* out;                                         // [N,Hq,D]
@@ -49,6 +50,9 @@ struct PagedParams {
 // ws_desc[2c], ws_desc[2c+1]: the unit that span c begins and a later one ends: {pieces, KV head, row tile, 0} and the
 // request's {first row, new tokens, 0, 0}; pieces == 0 when there is none. The first piece lies at slot 2c+1, the
 // pieces of the spans after it at slots 2(c+1), 2(c+2), ...
+
+// Row n of a request belongs to token n / G.
+__device__ __forceinline__ int paged_token(const PagedParams& p, int n) { return p.g_shift >= 0 ? n >> p.g_shift : n / p.G; }
 
 struct PagedRequest {
   int first, q, kv, pre;      // first row of the packed query, new tokens, keys, prefix; position of token i: kv - q + i
@@ -79,9 +83,9 @@ __device__ __forceinline__ int paged_hi(const PagedRequest& r, int i) { return m
 template <int ROWS, int KT>
 struct PagedUnit {
   int lo, hi, t0, n;
-  __device__ __forceinline__ void set(const PagedRequest& r, int G, int window, int tile) {
-    const int i0 = tile * ROWS / G, i1 = min(r.q - 1, (tile * ROWS + ROWS - 1) / G);
-    lo = paged_lo(r, window, i0);
+  __device__ __forceinline__ void set(const PagedParams& p, const PagedRequest& r, int tile) {
+    const int i0 = paged_token(p, tile * ROWS), i1 = min(r.q - 1, paged_token(p, tile * ROWS + ROWS - 1));
+    lo = paged_lo(r, p.window, i0);
     hi = max(paged_hi(r, i1), 0);
     if (hi <= lo) { lo = hi = 0; }
     t0 = lo / KT;
@@ -111,7 +115,7 @@ __device__ __forceinline__ int paged_lane_sum(const PagedParams& p, const PagedR
   if (tiles <= 4)
     for (int t = 0; t < tiles; ++t) {
       PagedUnit<ROWS, KT> u;
-      u.set(r, p.G, p.window, t);
+      u.set(p, r, t);
       sum += u.n;
     }
   unsigned big = __ballot_sync(0xffffffffu, tiles > 4);
@@ -123,7 +127,7 @@ __device__ __forceinline__ int paged_lane_sum(const PagedParams& p, const PagedR
     int part = 0;
     for (int t = lane; t < nt; t += 32) {
       PagedUnit<ROWS, KT> u;
-      u.set(rr, p.G, p.window, t);
+      u.set(p, rr, t);
       part += u.n;
     }
     part = __reduce_add_sync(0xffffffffu, part);
@@ -139,7 +143,7 @@ __device__ __forceinline__ int paged_find_tile(const PagedParams& p, const Paged
   for (int t0 = 0; t0 < nt; t0 += 32) {
     PagedUnit<ROWS, KT> u;
     u.n = 0;
-    if (t0 + lane < nt) u.set(r, p.G, p.window, t0 + lane);
+    if (t0 + lane < nt) u.set(p, r, t0 + lane);
     int inc = u.n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -198,7 +202,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedParams& p, int* s_sum
       sum = paged_lane_sum<ROWS, KT>(p, mine, lane);
     } else {
       PagedUnit<ROWS, KT> u;
-      u.set(mine, p.G, p.window, 0);
+      u.set(p, mine, 0);
       sum = tiles > 0 ? u.n : 0;
     }
     int inc = sum * p.Hkv;
@@ -359,27 +363,27 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// Scores of N neighbouring keys, the first at distance d0 = (key - position), in place: raw products q.k become
-// scores times log2(e). What they are made of is asked once per call, not per score.
+// N raw products q.k of one or more rows become scores times log2(e), in place; all lanes call. What they are made of
+// is asked once per call, not per score.
 //
 // tanh(y) = 1 - 2 / (1 + e^2y): its rounding is relative to 1, which is fp32 rounding of the largest of these scores
 // as long as that one is of the order of the cap. Where all 32 lanes' |y| are below 0.35, as scores far below their cap
 // are, the odd Taylor polynomial up to y^9 instead (first term left out: 0.00886 y^10 of the value, 2.5e-7), which also
 // leaves the exponential unit alone.
 template <int N>
-__device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, float slope_log2, int d0) {
+__device__ __forceinline__ void paged_scale(const PagedParams& p, float* x) {
   if (p.cap_log2 > 0.0f) {
     const uint64_t in2 = pack2(p.cap_in, p.cap_in);
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const uint64_t y = mul2(pack2(x[i], x[i + 1]), in2);
-      unpack2(y, x[i], x[i + 1]);
+      unpack2(mul2(pack2(x[i], x[i + 1]), in2), x[i], x[i + 1]);
       asm("max.f32 %0, %0, %1, %2;" : "+f"(big) : "f"(fabsf(x[i])), "f"(fabsf(x[i + 1])));
     }
+    const uint64_t cap2 = pack2(p.cap_log2, p.cap_log2);
     if (__any_sync(0xffffffffu, !(big < 0.35f))) {
       const uint64_t two2 = pack2(2.0f * PA_LOG2E, 2.0f * PA_LOG2E), m2 = pack2(-2.0f * p.cap_log2, -2.0f * p.cap_log2);
-      const uint64_t cap2 = pack2(p.cap_log2, p.cap_log2), one2 = pack2(1.0f, 1.0f);
+      const uint64_t one2 = pack2(1.0f, 1.0f);
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         float a, b;
@@ -388,7 +392,6 @@ __device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, flo
         unpack2(fma2(pack2(rcp(a), rcp(b)), m2, cap2), x[i], x[i + 1]);
       }
     } else {
-      const uint64_t cap2 = pack2(p.cap_log2, p.cap_log2);
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
         const uint64_t y = pack2(x[i], x[i + 1]), z = mul2(y, y);
@@ -404,24 +407,33 @@ __device__ __forceinline__ void paged_scores(const PagedParams& p, float* x, flo
 #pragma unroll
     for (int i = 0; i < N; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), scale2), x[i], x[i + 1]);
   }
-  if (p.slopes) {
-    // distances are whole numbers below 2^24, exact in fp32: four running pairs instead of a constant for each
-    constexpr int R = N >= 8 ? 4 : N / 2;
-    const bool behind = __any_sync(0xffffffffu, d0 + N > 1);     // some key behind its query: |p - j| is not p - j
-    const uint64_t s2 = behind ? pack2(-slope_log2, -slope_log2) : pack2(slope_log2, slope_log2);
-    const uint64_t step = pack2((float)(2 * R), (float)(2 * R));
-    uint64_t d[R];
+}
+// The distance term of N neighbouring keys, the first at distance d0 = key - position. Distances are whole numbers below
+// 2^24, exact in fp32: four running pairs instead of a constant for each.
+template <int N>
+__device__ __forceinline__ void paged_bias(float* x, float slope_log2, int d0) {
+  constexpr int R = N >= 8 ? 4 : N / 2;
+  const bool behind = __any_sync(0xffffffffu, d0 + N > 1);       // some key behind its query: |p - j| is not p - j
+  const float s = behind ? -slope_log2 : slope_log2;
+  const uint64_t s2 = pack2(s, s), step = pack2((float)(2 * R), (float)(2 * R));
+  const float f0 = (float)d0;
+  uint64_t d[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) d[i] = pack2((float)(d0 + 2 * i), (float)(d0 + 2 * i + 1));
+  for (int i = 0; i < R; ++i) d[i] = pack2(f0 + (float)(2 * i), f0 + (float)(2 * i + 1));
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      float a, b;
-      unpack2(d[i % R], a, b);
-      if (behind) { a = fabsf(a); b = fabsf(b); }
-      unpack2(fma2(pack2(a, b), s2, pack2(x[2 * i], x[2 * i + 1])), x[2 * i], x[2 * i + 1]);
-      if (i + R < N / 2) d[i % R] = add2(d[i % R], step);
-    }
+  for (int i = 0; i < N / 2; ++i) {
+    float a, b;
+    unpack2(d[i % R], a, b);
+    if (behind) { a = fabsf(a); b = fabsf(b); }
+    unpack2(fma2(pack2(a, b), s2, pack2(x[2 * i], x[2 * i + 1])), x[2 * i], x[2 * i + 1]);
+    if (i + R < N / 2) d[i % R] = add2(d[i % R], step);
   }
+}
+// Bit i: whether key t + i lies in [lo, hi), for 32 keys.
+__device__ __forceinline__ uint32_t paged_seen(int t, int lo, int hi) {
+  const int a = min(max(lo - t, 0), 32), b = min(max(hi - t, 0), 32);
+  const uint32_t below = a < 32 ? (1u << a) - 1u : 0xffffffffu, upto = b < 32 ? (1u << b) - 1u : 0xffffffffu;
+  return upto & ~below;
 }
 
 template <typename T>
@@ -472,51 +484,83 @@ __global__ void __launch_bounds__(PM_WARPS * 32) paged_merge_kernel(PagedParams 
   if (n == 0) return;
   const int rows = min(ROWS, e.y * p.G - d.z * ROWS);
   const int row0 = (blockIdx.y * PM_WARPS + warp) * RPW;
+  if (row0 >= rows) return;
   constexpr int E = D / 32;
   auto slot = [&](int s) -> int64_t { return s == 0 ? 2 * c + 1 : 2 * (c + s); };
-  for (int rr = row0; rr < min(row0 + RPW, rows); ++rr) {
-    float m = -INFINITY, l = 0.0f, acc[E];
+  // the warp's rows side by side, so that a round trip serves all of them
+  float m[RPW], l[RPW], acc[RPW][E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = 0.0f;
-    for (int s0 = 0; s0 < n; s0 += 32) {
-      const float2 ml = s0 + lane < n ? p.ws_ml[slot(s0 + lane) * ROWS + rr] : make_float2(-INFINITY, 0.0f);
-      float top = ml.x;
+  for (int q = 0; q < RPW; ++q) {
+    m[q] = -INFINITY;
+    l[q] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[q][i] = 0.0f;
+  }
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    float2 ml[RPW];
+    float w[RPW];
+#pragma unroll
+    for (int q = 0; q < RPW; ++q)
+      ml[q] = s0 + lane < n && row0 + q < rows ? p.ws_ml[slot(s0 + lane) * ROWS + row0 + q] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+    for (int q = 0; q < RPW; ++q) {
+      float top = ml[q].x;
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float mn = fmaxf(m, top), ms = mn == -INFINITY ? 0.0f : mn;
-      const float old = exp2f(m - ms), w = exp2f(ml.x - ms);
-      float part = w * ml.y;
+      const float mn = fmaxf(m[q], top), ms = mn == -INFINITY ? 0.0f : mn;
+      const float old = exp2f(m[q] - ms);
+      w[q] = exp2f(ml[q].x - ms);
+      float part = w[q] * ml[q].y;
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      l = fmaf(l, old, part);
-      m = mn;
+      l[q] = fmaf(l[q], old, part);
+      m[q] = mn;
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] *= old;
-      const int k = min(32, n - s0);
-#pragma unroll 8
-      for (int s = 0; s < k; ++s) {
-        const float* o = p.ws_o + (slot(s0 + s) * ROWS + rr) * D + lane * E;
-        const float f = __shfl_sync(0xffffffffu, w, s);
-        if constexpr (E == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(o);
-          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
-          acc[2] = fmaf(f, v.z, acc[2]); acc[3] = fmaf(f, v.w, acc[3]);
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(o);
-          acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]);
-        }
-      }
+      for (int i = 0; i < E; ++i) acc[q][i] *= old;
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);       // a NaN stays one
-    const int flat = d.z * ROWS + rr, token = flat / p.G, head = d.y * p.G + (flat - token * p.G);
+    const int k = min(32, n - s0);
+    constexpr int U = 16 / RPW;
+#pragma unroll 1
+    for (int s1 = 0; s1 < k; s1 += U) {
+      float v[U][RPW][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int q = 0; q < RPW; ++q) {
+          const bool have = s1 + u < k && row0 + q < rows;
+          const float* o = p.ws_o + (slot(s0 + s1 + u) * ROWS + row0 + q) * D + lane * E;
+          if constexpr (E == 4) {
+            const float4 t = have ? *reinterpret_cast<const float4*>(o) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[u][q][0] = t.x; v[u][q][1] = t.y; v[u][q][2] = t.z; v[u][q][3] = t.w;
+          } else {
+            const float2 t = have ? *reinterpret_cast<const float2*>(o) : make_float2(0.0f, 0.0f);
+            v[u][q][0] = t.x; v[u][q][1] = t.y;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int q = 0; q < RPW; ++q) {
+          const float f = __shfl_sync(0xffffffffu, w[q], (s1 + u) & 31);
+          if (s1 + u < k)
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[q][i] = fmaf(f, v[u][q][i], acc[q][i]);
+        }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < RPW; ++q) {
+    if (row0 + q >= rows) break;
+    const float inv = l[q] > 0.0f ? 1.0f / l[q] : (l[q] == 0.0f ? 0.0f : l[q]);       // a NaN stays one
+    const int flat = d.z * ROWS + row0 + q, token = paged_token(p, flat), head = d.y * p.G + (flat - token * p.G);
     const int64_t at = (int64_t)(e.x + token) * p.Hq + head;
     T* out = reinterpret_cast<T*>(p.out) + at * D + lane * E;
     if constexpr (E == 4) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(Half2Of<T>::pack(acc[0] * inv, acc[1] * inv), Half2Of<T>::pack(acc[2] * inv, acc[3] * inv));
+      *reinterpret_cast<uint2*>(out) = make_uint2(Half2Of<T>::pack(acc[q][0] * inv, acc[q][1] * inv), Half2Of<T>::pack(acc[q][2] * inv, acc[q][3] * inv));
     } else {
-      *reinterpret_cast<uint32_t*>(out) = Half2Of<T>::pack(acc[0] * inv, acc[1] * inv);
+      *reinterpret_cast<uint32_t*>(out) = Half2Of<T>::pack(acc[q][0] * inv, acc[q][1] * inv);
     }
-    if (p.lse && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : ((m == -INFINITY ? 0.0f : m) + log2f(l)) * PA_LN2;
+    if (p.lse && lane == 0) p.lse[at] = l[q] == 0.0f ? -INFINITY : ((m[q] == -INFINITY ? 0.0f : m[q]) + log2f(l[q])) * PA_LN2;
   }
 }
 

@@ -934,7 +934,7 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     query = _aligned_rows(query)
     device = query.device
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=dtype, device=device)
+        out = query.new_empty((N, Hq, D))
     lse = torch.empty((N, Hq), dtype=torch.float32, device=device) if return_lse else None
     if N == 0:
         return (out, lse) if return_lse else out
