@@ -668,7 +668,8 @@ int kvb_decode_step(const kvb_decode_step_params* p, int device, void* stream);
  *                   [0, num_pages], more pages given back than there are). Unless all four are 0
  *                   nothing changes: no page moves, cu_q is all 0, the slots are -1, lengths and
  *                   count are copied.
- * Negative lengths count as 0.
+ * Negative lengths count as 0. A page belongs to one request: one that several table rows name (a shared
+ * prefix) may be read by all of them, but must not be given back by more than one. W * page_tokens <= 2^30.
  * ------------------------------------------------------------------------------------- */
 int kvb_page_plan(const int32_t* kv_len, const int32_t* q_len, const uint8_t* finished, int B,
                   int32_t* page_table, int64_t page_table_stride, int W,

@@ -227,7 +227,7 @@ class RequestPagedKV:
     the device and can be captured into a graph (``q_len`` and ``finished`` are then buffers the caller refills).
 
         kv = RequestPagedKV(layers, max_requests, Hkv, D, page_tokens, num_pages, pages_per_request, device)
-        plan = kv.step(q_len, capacity)                   # q_len int32 [max_requests], 0 where a request is idle
+        plan = kv.step(q_len, capacity, max_q=1)          # q_len int32 [max_requests], 0 where a request is idle
         for layer in range(layers):                       # rows of the step: plan.request, plan.position
             kv.append(layer, key_rows, value_rows)        # [capacity, Hkv, D]
             out = kv.attend(layer, query)                 # [capacity, Hq, D]
@@ -246,10 +246,14 @@ class RequestPagedKV:
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
         self.plan: Optional[ops.PagePlan] = None
+        self.max_q = 0
 
-    def step(self, q_len: torch.Tensor, capacity: int, finished: Optional[torch.Tensor] = None) -> ops.PagePlan:
+    def step(self, q_len: torch.Tensor, capacity: int, finished: Optional[torch.Tensor] = None,
+             max_q: int = 0) -> ops.PagePlan:
         """Retires the ``finished`` requests and makes room for ``q_len[b]`` new tokens of every request (a finished
-        one starts over). ``capacity`` bounds their sum. The plan's ``status`` says whether there was room."""
+        one starts over). ``capacity`` bounds their sum. ``max_q``: the largest ``q_len`` when the caller knows it (a decode
+        step: 1); ``attend`` then takes the kernel made for it. The plan's ``status`` says whether there was room."""
+        self.max_q = int(max_q)
         self.plan = ops.page_plan(self.kv_len, q_len, self.page_table, self.free_pages, self.free_count, self.page_tokens,
                                   capacity, finished=finished, in_place=True)
         return self.plan
@@ -266,4 +270,4 @@ class RequestPagedKV:
     def attend(self, layer: int, query: torch.Tensor, **kwargs):
         """``ops.paged_attend`` of the step's tokens ``[capacity, Hq, D]`` over their requests."""
         return ops.paged_attend(query, self.key_pools[layer], self.value_pools[layer], self.page_table, self.kv_len,
-                                cu_q=self._planned().cu_q, **kwargs)
+                                cu_q=self._planned().cu_q, max_q=self.max_q, **kwargs)

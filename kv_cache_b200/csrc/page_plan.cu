@@ -205,7 +205,7 @@ extern "C" __attribute__((visibility("default"))) int kvb_page_plan(
       !slot || !position || !request || !status)
     return KVB_BAD_ARG;
   if (B < 1 || B > PLAN_MAX_B || W < 1 || num_pages < 1 || capacity < 1 || capacity > (1 << 30) ||
-      page_table_stride < W || !page_tokens_ok(page_tokens))
+      page_table_stride < W || !page_tokens_ok(page_tokens) || (int64_t)W * page_tokens > 0x40000000)
     return KVB_BAD_SHAPE;
   if (!aligned_to(slot, 8)) return KVB_BAD_ALIGN;
   DeviceGuard guard(device);

@@ -445,7 +445,8 @@ extern "C" __attribute__((visibility("default"))) int kvb_paged_attend(const kvb
   if (a->max_q < 0) return KVB_BAD_ARG;
   if (a->page_table_stride < a->W || (a->cu_q == nullptr && a->N != a->B)) return KVB_BAD_SHAPE;
   if (a->elem_type != 0 && a->elem_type != 1) return KVB_BAD_ARG;
-  if (!(a->scaling > 0.0f) || a->scaling > 3.0e38f || !(a->softcap >= 0.0f) || a->softcap > 3.0e38f || a->window < 0)
+  if (!(a->scaling > 0.0f) || a->scaling > 3.0e38f || !(a->softcap >= 0.0f) || a->softcap > 3.0e38f || a->window < 0 ||
+      (a->softcap > 0.0f && !(a->scaling / a->softcap < 3.0e38f)))
     return KVB_BAD_ARG;
   const int64_t strides[] = {a->q_st, a->q_sh, a->k_sp, a->k_sh, a->k_st, a->v_sp, a->v_sh, a->v_st};
   for (int64_t s : strides)

@@ -68,8 +68,12 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
     r.first = b;
     r.q = 1;
   }
-  const int64_t most = (int64_t)p.W << p.shift;
-  r.kv = (int)min((int64_t)max(p.kv_len[b], 0), most);
+  const int most = p.W << p.shift;                     // at most 2^30
+  r.kv = max(p.kv_len[b], 0);
+  if (r.kv > most) {
+    r.kv = most;
+    atomicExch(&g_device_status, (int)KVB_BAD_ARG);
+  }
   r.pre = p.prefix ? min(max(p.prefix[b], 0), r.kv) : 0;
   return r;
 }
@@ -408,8 +412,8 @@ __device__ __forceinline__ void paged_scale(const PagedParams& p, float* x) {
     for (int i = 0; i < N; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), scale2), x[i], x[i + 1]);
   }
 }
-// The distance term of N neighbouring keys, the first at distance d0 = key - position. Distances are whole numbers below
-// 2^24, exact in fp32: four running pairs instead of a constant for each.
+// The distance term of N neighbouring keys, the first at distance d0 = key - position. Distances are whole numbers, exact in
+// fp32 up to 2^24: four running pairs instead of a constant for each.
 template <int N>
 __device__ __forceinline__ void paged_bias(float* x, float slope_log2, int d0) {
   constexpr int R = N >= 8 ? 4 : N / 2;

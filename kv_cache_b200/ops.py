@@ -788,6 +788,9 @@ def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tenso
     count are returned, and with ``in_place`` written to ``kv_len`` and ``free_count`` themselves (a captured step).
     ``capacity``: size of the per-token outputs, at least the number of new tokens.
 
+    A page belongs to one request: several table rows may name it for ``paged_attend`` (a shared prefix), but only one of
+    them may ever finish.
+
     ``status`` of the result: pages lacking, tokens beyond ``capacity``, requests whose table row is too short, 1 if
     the stack or a finished length cannot be. Unless all are 0 nothing is changed and no token has a slot."""
     dev = kv_len.get_device()
@@ -924,7 +927,8 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
         _device_ints("slopes", slopes, Hq, dev, torch.float32)
     scaling = float(D) ** -0.5 if scaling is None else float(scaling)
     softcap, window, max_q = float(softcap), int(window), int(max_q)
-    if not 0.0 < scaling < 3.0e38 or not 0.0 <= softcap < 3.0e38 or window < 0 or max_q < 0:
+    if not 0.0 < scaling < 3.0e38 or not 0.0 <= softcap < 3.0e38 or window < 0 or max_q < 0 \
+            or (softcap and scaling > 3.0e38 * softcap):
         raise RuntimeError("scaling must be positive and finite, softcap, window and max_q not negative")
     if out is not None and (out.shape != query.shape or out.dtype != dtype or not out.is_contiguous()
                             or out.get_device() != dev or out.data_ptr() & 15):

@@ -54,7 +54,7 @@ def same_plan(p, t, want, table, free):
 
 
 @pytest.mark.parametrize("B,P,q_hi,len_hi", [(1, 16, 1, 0), (1, 1, 5, 3), (3, 16, 40, 50), (33, 64, 300, 700), (256, 16, 1, 300),
-                                             (1025, 8, 3, 20), (2500, 4, 9, 6), (5, 256, 6000, 100), (70, 32, 600, 3000)])
+                                             (1025, 8, 3, 20), (2500, 4, 9, 6), (5, 256, 6000, 100), (70, 32, 600, 3000), (8192, 4, 2, 9)])
 @pytest.mark.parametrize("done", [True, False])
 def test_plan(cuda_device, B, P, q_hi, len_hi, done):
     kv, q, table, free, count, fin = plan_inputs(B, P, q_hi, len_hi, seed=B * 31 + P)
@@ -257,6 +257,28 @@ def test_bad_device_data_is_reported_and_harms_nothing(cuda_device, max_q):
     device_status(cuda_device)
 
 
+@pytest.mark.parametrize("max_q", [1, 40])
+def test_requests_that_share_pages(cuda_device, max_q):
+    """A common prefix stored once: two table rows name the same pages."""
+    q, kv = [40, 3], [200, 163]
+    t, key, value = ref.paged_case(cuda_device, q, kv, 4, 2, 64, 32, torch.float16, seed=6)
+    t["page_table"][1, :5] = t["page_table"][0, :5]
+    for x in (key, value):
+        x[1] = torch.cat((x[0][:, :160], x[1][:, 160:]), 1)
+    got = ops.paged_attend(t["query"], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"], cu_q=t["cu_q"], max_q=max_q)
+    want, _, bound, _ = ref.attend(t["query"], key, value, q, kv, 64 ** -0.5)
+    assert ((got.double().cpu() - want).abs() <= bound).all()
+
+
+def test_lengths_beyond_the_table_are_cut_and_reported(cuda_device):
+    t, key, value = ref.paged_case(cuda_device, [1, 1], [64, 40], 4, 2, 64, 32, torch.float16, seed=7)
+    want = ops.paged_attend(t["query"], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"])
+    assert device_status(cuda_device) == 0
+    t["kv_len"][0] = 65
+    got = ops.paged_attend(t["query"], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"])
+    assert device_status(cuda_device) == 7 and torch.equal(got, want)
+
+
 def test_strided_operands(cuda_device):
     """Queries that are columns of a fused projection, pools with tokens outside heads, a table cut from a wider one."""
     q, kv = [1, 60, 7], [90, 200, 7]
@@ -344,8 +366,8 @@ def test_offsets_beyond_32_bits(cuda_device):
 
 # ---- a run of them together ----------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("captured", [False, True])
-def test_serving_run(cuda_device, captured):
+@pytest.mark.parametrize("captured,max_q", [(False, 0), (True, 0), (True, 1)])
+def test_serving_run(cuda_device, captured, max_q):
     """Requests come, grow by chunks and single tokens, end, and their rows and pages are used again: every step's
     output equals the 64-bit attention over what each request was given. Two layers share the plan."""
     Hq, Hkv, D, P, B, layers, capacity = 6, 2, 64, 8, 5, 2, 80
@@ -359,7 +381,7 @@ def test_serving_run(cuda_device, captured):
     outs = torch.zeros((layers, capacity, Hq, D), dtype=dtype, device=cuda_device)
 
     def body():
-        kv.step(q_len, capacity, finished=done)
+        kv.step(q_len, capacity, finished=done, max_q=max_q)
         for layer in range(layers):
             x = ins[layer]
             kv.append(layer, x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:])

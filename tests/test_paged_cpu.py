@@ -60,7 +60,7 @@ def attend_args(**kw):
     dict(query=torch.zeros((3, 4, 64))), dict(query=torch.zeros((3, 4, 64), dtype=torch.float16)), dict(query=torch.zeros((3, 3, 64), dtype=torch.bfloat16)),
     dict(query=torch.zeros((2, 4, 64), dtype=torch.bfloat16)), dict(query=torch.zeros((3, 4, 1, 64), dtype=torch.bfloat16)), dict(kv_len=torch.ones(3)),
     dict(cu_q=torch.zeros(3, **i32)), dict(slopes=torch.zeros(2)), dict(slopes=torch.zeros(4, dtype=torch.float64)), dict(prefix_len=torch.zeros(4, **i32)),
-    dict(scaling=0.0), dict(scaling=-1.0), dict(scaling=float("nan")), dict(scaling=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(window=-1), dict(max_q=-1),
+    dict(scaling=0.0), dict(scaling=-1.0), dict(scaling=float("nan")), dict(scaling=float("inf")), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=1e-39, scaling=1.0), dict(window=-1), dict(max_q=-1),
     dict(out=torch.zeros((3, 4, 64))), dict(out=torch.zeros((2, 4, 64), dtype=torch.bfloat16)),
     dict(query=torch.zeros((3, 4, 32), dtype=torch.bfloat16), key_pool=torch.zeros((4, 2, 8, 32), dtype=torch.bfloat16), value_pool=torch.zeros((4, 2, 8, 32), dtype=torch.bfloat16)),
     dict()])
@@ -86,7 +86,7 @@ def test_c_refusals_without_a_device():
     assert attend() == 3                                  # every other check passed: there is no device 999
     assert lib.kvb_paged_attend(None, 0, None) == 7
     for bad in (dict(query=None), dict(workspace=None), dict(elem_type=2), dict(scaling=0.0), dict(scaling=float("nan")), dict(softcap=-1.0),
-                dict(window=-1)):
+                dict(softcap=1e-39), dict(window=-1), dict(max_q=-1)):
         assert attend(**bad) == 7, bad
     for bad in (dict(D=96), dict(Hq=5), dict(B=0), dict(B=8193), dict(N=2), dict(page_tokens=12), dict(W=0), dict(page_table_stride=1),
                 dict(N=-1), dict(num_pages=0), dict(W=1 << 28)):
@@ -100,7 +100,7 @@ def test_c_refusals_without_a_device():
         return lib.kvb_page_plan(a, a, None, B, table, stride, W, a, num, a, P, cap, a, a, a, a, a, a, a, 999, None)
 
     assert plan() == 3 and plan(table=None) == 7
-    assert [plan(B=0), plan(B=8193), plan(W=3), plan(num=0), plan(P=3), plan(cap=0)] == [1] * 6
+    assert [plan(B=0), plan(B=8193), plan(W=3), plan(num=0), plan(P=3), plan(cap=0), plan(W=1 << 20, stride=1 << 20, P=2048)] == [1] * 7
 
     def append(D=64, N=5, st=128, k=a, P=8):
         return lib.kvb_paged_append(k, st, 64, a, 128, 64, a, N, 2, D, a, 1024, 512, 64, a, 1024, 512, 64, 4, P, 999, None)
