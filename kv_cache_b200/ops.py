@@ -814,11 +814,10 @@ def page_plan(kv_len: torch.Tensor, q_len: torch.Tensor, page_table: torch.Tenso
     if dev < 0:
         _dev(kv_len)
     if out is None:
-        # one allocation for the 32-bit outputs: a step's plan is made once and short
-        ints = torch.empty(2 * B + 6 + 2 * capacity, dtype=torch.int32, device=kv_len.device)
-        cu, now, left, pos, req, status = ints.split((B + 1, B, 1, capacity, capacity, 4))
-        slot = torch.empty(capacity, dtype=torch.int64, device=kv_len.device)
-        out = PagePlan(cu, kv_len if in_place else now, free_count if in_place else left, slot, pos, req, status)
+        # one allocation for all outputs (the 64-bit one first): seven would take longer than the kernel
+        ints = kv_len.new_empty(2 * B + 6 + 4 * capacity)
+        slot, cu, now, left, pos, req, status = torch.split_with_sizes(ints, (2 * capacity, B + 1, B, 1, capacity, capacity, 4))
+        out = PagePlan(cu, kv_len if in_place else now, free_count if in_place else left, slot.view(torch.int64), pos, req, status)
     else:
         if in_place and (out.kv_len is not kv_len or out.free_count is not free_count):
             raise RuntimeError("in_place needs the plan's own kv_len and free_count")
@@ -938,8 +937,8 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     query = _aligned_rows(query)
     device = query.device
     if out is None:
-        out = query.new_empty((N, Hq, D))
-    lse = torch.empty((N, Hq), dtype=torch.float32, device=device) if return_lse else None
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    lse = torch.empty_strided((N, Hq), (Hq, 1), dtype=torch.float32, device=device) if return_lse else None
     if N == 0:
         return (out, lse) if return_lse else out
     lib = _native.lib()
@@ -947,7 +946,7 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
     ws_bytes = lib.kvb_paged_attend_workspace_bytes(N, B, Hq, Hkv, W, P, D, max_q)
     if ws_bytes == 0:
         raise RuntimeError("kvb_paged_attend: unsupported shape")
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+    ws = torch.empty_strided((ws_bytes,), (1,), dtype=torch.uint8, device=device)
     q0, q1, _ = query.stride()
     p = PagedAttendParams(                               # in the order of the struct
         query.data_ptr(), q0, q1, key_pool.data_ptr(), ks[0], ks[1], ks[2], value_pool.data_ptr(), vs[0], vs[1], vs[2],
