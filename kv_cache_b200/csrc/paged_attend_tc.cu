@@ -11,7 +11,8 @@ namespace kvb {
 
 constexpr int PT_ROWS = 256;                // rows of a unit: two accumulator tiles of 128
 constexpr int PT_MAX_GRID = 148;            // one block per SM
-constexpr int PT_SNAP = 2, PT_LEAST = 3;    // key tiles: see paged_common.cuh
+constexpr int PT_SNAP = 1, PT_LEAST = 1;    // key tiles, see paged_common.cuh: a short call (2 prompts, 333 tokens) takes 22.8 us,
+                                            // 25.7 with 2 and 3, 34.7 with 3 and 5; long ones do not differ
 constexpr int PT_KT = 128;                  // keys per tile
 constexpr int PT_THREADS = 384;             // warps 0-3, 4-7: softmax of row tile 0, 1; 8, 9: loads; 10: MMA issue
 constexpr int PT_HALF = 128 * 128;          // bytes of 128 rows x 64 16-bit elements, 128-byte swizzle
@@ -344,9 +345,8 @@ struct PtLoader {
 
 // ---- MMA issue: one warp, one elected lane -----------------------------------------------------------------
 // Descriptors differ from a constant only in their address word. The whole warp walks the loop with values that are
-// the same in every lane (votes and shuffles say so to the compiler), so they stay in uniform registers, from which the
-// instruction takes them; with one lane inside a branch every descriptor was moved there first, and the issue loop of a
-// tile pair alone took 6000 cycles.
+// the same in every lane (votes and shuffles say so to the compiler) and elects a lane around each group of products:
+// a lane chosen by its number made the compiler branch around every single product (3660 instead of 4420 cycles a tile pair).
 template <typename T, int D>
 __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, uint32_t tmem_, PagedPlace at, PagedRequest r, long long left) {
   using Cfg = PtCfg<D>;
@@ -455,7 +455,7 @@ __device__ __forceinline__ void pt_issue(const PagedParams& p, uint32_t base_, u
     if (left <= 0 || !paged_next<PT_ROWS>(p, at, r)) break;
   }
   commit(base + Cfg::DONE);
-  pt_wait(base + Cfg::DONE, 0, dead);
+  pt_wait(base + Cfg::DONE, 0, base + Cfg::OFF_MISC + 8);  // no product may run on after tensor memory is given back
 }
 
 // ---- softmax of one row tile: 4 warps, one row per thread ------------------------------------------------
@@ -497,7 +497,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
         continue;
       }
       // Pass 1: the largest score. Scores that are changed (capped, biased, masked) go back to their place. Reading the
-      // tile twice costs less than holding its 128 scores, which leaves the other roles too few registers.
+      // tile twice costs less than holding its 128 scores: registers would spill.
       const int t0 = n * PT_KT;
       const bool edge = t0 < all_lo || t0 + PT_KT > all_hi;
       uint32_t v[2][32];
@@ -652,13 +652,19 @@ __device__ __forceinline__ void pt_own(PagedPlace& at, PagedRequest& r, long lon
   asm volatile("" : "+r"(at.b), "+r"(at.h), "+r"(at.tile), "+r"(at.k), "+r"(r.first), "+r"(r.q), "+r"(r.kv), "+r"(r.pre), "+l"(left));
 }
 
-// A block walks its span unit by unit: 4 warps copy K and V tiles (and each unit's query rows) into shared memory in the
-// 128-byte-swizzled layout, one thread issues S_w = Q_w K^T and O_w += P_w V for two row tiles w of 128 rows, and four
+// A block walks its span unit by unit: two warps bring K and V tiles (and each unit's query rows) into shared memory in the
+// 128-byte-swizzled layout, one warp issues S_w = Q_w K^T and O_w += P_w V for two row tiles w of 128 rows, and four
 // warps per row tile, one row per thread, turn scores into weights: S_w is read from tensor memory, P_w goes back over
 // it as 16-bit operand of the second product, and O_w stays in tensor memory until the unit ends. While the softmax of
 // one row tile runs, the tensor core works on the other. The reference of a row moves only when a score passes it by
 // 2^8, so O_w is rescaled rarely, and then by the softmax warps, which know from the order of issue that the previous
-// product is complete. Rows of K and V outside what the unit sees are zero-filled, not read.
+// product is complete. Weights are rounded to the input type for the second product, as the values they weigh are; their
+// sum is taken before that. Rows of K and V that no token of the request sees are zero-filled, not read.
+//
+// 384 threads so that a block's 65536 registers give 208 to a softmax thread and 88 to the others: with
+// 512 threads spills in the issuing warp cost a quarter of the time. Measured, bf16: 2048 tokens on 30720 cached, 32/8 heads
+// (1.07 TFLOP) 0.94-0.98 ms = 1090-1138 TFLOP/s, 0.66-0.69 of the cuBLAS burst rate (1.07 ms under the power cap): 3650
+// cycles per pair of row tiles and key tile, of which the products fill 2048 and the 32768 exponentials, 16 a cycle, 2048.
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -703,6 +709,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     fence_mbar_init();
   }
   PagedRequest r = paged_request(p, at.b);
+  fence_proxy_async_smem();                              // the scheduler's scratch is written by the TMA engine next
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -477,7 +477,8 @@ __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst_smem, const voi
 // Joins the pieces of the units that a cut divided: block (c, y) takes the unit that span c leaves unfinished,
 // rows y*RB ... of its tile, one warp per row:
 //     M = max m_s,  out = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
-// Bound by round trips to L2: the descriptor, then (m, l) of up to 32 pieces at once and the outputs beside them.
+// Bound by round trips to L2: the descriptor, then (m, l) of up to 32 pieces at once and the outputs of 16 (rows x pieces)
+// at a time; 3-10 us.
 constexpr int PM_WARPS = 4;
 template <typename T, int D, int ROWS, int RPW>
 __global__ void __launch_bounds__(PM_WARPS * 32) paged_merge_kernel(PagedParams p) {

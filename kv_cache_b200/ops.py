@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -883,6 +884,11 @@ def paged_append(key_rows: torch.Tensor, value_rows: torch.Tensor, slot: torch.T
         value_pool.data_ptr(), vs[0], vs[1], vs[2], num_pages, P, dev, _raw_stream(dev)), "kvb_paged_append")
 
 
+@lru_cache(maxsize=4096)
+def _paged_workspace_bytes(*shape: int) -> int:
+    return _native.lib().kvb_paged_attend_workspace_bytes(*shape)
+
+
 def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, page_table: torch.Tensor,
                  kv_len: torch.Tensor, *, cu_q: Optional[torch.Tensor] = None, max_q: int = 0,
                  scaling: Optional[float] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
@@ -943,7 +949,7 @@ def paged_attend(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.
         return (out, lse) if return_lse else out
     lib = _native.lib()
     W = page_table.shape[1]
-    ws_bytes = lib.kvb_paged_attend_workspace_bytes(N, B, Hq, Hkv, W, P, D, max_q)
+    ws_bytes = _paged_workspace_bytes(N, B, Hq, Hkv, W, P, D, max_q)
     if ws_bytes == 0:
         raise RuntimeError("kvb_paged_attend: unsupported shape")
     ws = torch.empty_strided((ws_bytes,), (1,), dtype=torch.uint8, device=device)
