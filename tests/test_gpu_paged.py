@@ -329,6 +329,35 @@ def test_repeatable_on_another_stream_and_in_graphs(cuda_device, max_q):
     assert all(torch.equal(want, o) for o in outs)
 
 
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_two_streams_at_once(cuda_device, max_q):
+    """Calls in flight on two streams do not disturb each other (each has its own workspace)."""
+    cases = []
+    for seed, (q, kv) in enumerate([([1, 3, 64], [3000, 40, 1500]), ([64, 1, 1], [900, 2100, 33])]):
+        t, _, _ = ref.paged_case(cuda_device, q, kv, 8, 2, 128, 16, torch.bfloat16, seed=seed)
+        call = lambda t=t: ops.paged_attend(t["query"], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"],  # noqa: E731
+                                            cu_q=t["cu_q"], max_q=max_q)
+        cases.append((call, call(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, (call, _, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                outs[i].append(call())
+    torch.cuda.synchronize()
+    for (_, want, _), got in zip(cases, outs):
+        assert all(torch.equal(want, o) for o in got)
+
+
+def test_query_rows_that_are_not_aligned(cuda_device):
+    t, _, _ = ref.paged_case(cuda_device, [1, 20], [90, 20], 8, 2, 128, 16, torch.float16, seed=1)
+    want = ops.paged_attend(t["query"], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"], cu_q=t["cu_q"])
+    wide = torch.zeros((*t["query"].shape[:2], 131), dtype=torch.float16, device=cuda_device)
+    wide[..., 1:129] = t["query"]
+    got = ops.paged_attend(wide[..., 1:129], t["key_pool"], t["value_pool"], t["page_table"], t["kv_len"], cu_q=t["cu_q"])
+    assert torch.equal(want, got)
+
+
 def test_many_requests(cuda_device):
     r = random.Random(1)
     B = 1500
