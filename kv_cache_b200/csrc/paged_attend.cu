@@ -11,8 +11,7 @@ constexpr int PR_KT = 16 * PR_WARPS;        // keys of a tile, 16 per warp
 constexpr int PR_STAGES = 3;
 constexpr int PR_SNAP = 1, PR_LEAST = 4;    // key tiles, see paged_common.cuh: 4096 keys x 8 heads 14.4 us, 14.9 with 2, 15.5 with 8
 constexpr int PR_MAX_GRID = 296;            // two blocks per SM
-constexpr float PR_SHIFT = 7.0f;            // the reference of a row lies 2^7 above zero weight: fresh weights reach
-constexpr float PR_LAZY = 8.0f;             // 2^7, stale ones 2^15, inside fp16's range; small ones keep its normal bits
+constexpr float PR_LAZY = 8.0f;             // a row's reference moves when a score passes it by 2^8
 
 template <int D>
 struct RowsCfg {
@@ -203,13 +202,13 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
         mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 1));
         mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 2));
       }
-      const bool move0 = mx[0] - PR_SHIFT > m[0] + PR_LAZY, move1 = mx[1] - PR_SHIFT > m[1] + PR_LAZY;
+      const bool move0 = mx[0] > m[0] + PR_LAZY, move1 = mx[1] > m[1] + PR_LAZY;
       if (__any_sync(0xffffffffu, move0 || move1)) {
         float a[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const bool mv = w == 0 ? move0 : move1;
-          const float mn = mv ? mx[w] - PR_SHIFT : m[w];
+          const float mn = mv ? mx[w] : m[w];
           a[w] = mv ? exp2f(m[w] - mn) : 1.0f;
           m[w] = mn;
           l[w] *= a[w];
@@ -228,11 +227,12 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
           x[n][e] = ex2(x[n][e] - ms[e >> 1]);
           l[e >> 1] += x[n][e];
         }
+      constexpr float W = Half2Of<T>::WEIGHT;
       uint32_t pa[4];
-      pa[0] = Half2Of<T>::pack(x[0][0], x[0][1]);
-      pa[1] = Half2Of<T>::pack(x[0][2], x[0][3]);
-      pa[2] = Half2Of<T>::pack(x[1][0], x[1][1]);
-      pa[3] = Half2Of<T>::pack(x[1][2], x[1][3]);
+      pa[0] = Half2Of<T>::pack(W * x[0][0], W * x[0][1]);
+      pa[1] = Half2Of<T>::pack(W * x[0][2], W * x[0][3]);
+      pa[2] = Half2Of<T>::pack(W * x[1][0], W * x[1][1]);
+      pa[3] = Half2Of<T>::pack(W * x[1][2], W * x[1][3]);
 #pragma unroll
       for (int n = 0; n < KS; ++n) {
         // matrices: keys 0-7 | 8-15 | 0-7 | 8-15, d pieces 2n | 2n | 2n+1 | 2n+1
@@ -274,8 +274,9 @@ __global__ void __launch_bounds__(PR_THREADS, 2) paged_rows_kernel(PagedParams p
 #pragma unroll
       for (int w = 0; w < PR_WARPS; ++w) {
         const float2 ml = s_ml[w][row];
-        const float f = exp2f(ml.x - ms);
+        float f = exp2f(ml.x - ms);
         L = fmaf(f, ml.y, L);
+        f *= 1.0f / Half2Of<T>::WEIGHT;
         const float* src = reinterpret_cast<const float*>(pr_smem + w * Cfg::WARPB) + row * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(f, src[e], acc[e]);

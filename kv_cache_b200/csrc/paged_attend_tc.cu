@@ -16,8 +16,7 @@ constexpr int PT_SNAP = 1, PT_LEAST = 1;    // key tiles, see paged_common.cuh: 
 constexpr int PT_KT = 128;                  // keys per tile
 constexpr int PT_THREADS = 384;             // warps 0-3, 4-7: softmax of row tile 0, 1; 8, 9: loads; 10: MMA issue
 constexpr int PT_HALF = 128 * 128;          // bytes of 128 rows x 64 16-bit elements, 128-byte swizzle
-constexpr float PT_SHIFT = 7.0f;            // as in the kernel for few rows: weights reach 2^7, stale ones 2^15
-constexpr float PT_LAZY = 8.0f;
+constexpr float PT_LAZY = 8.0f;             // a row's reference moves when a score passes it by 2^8
 
 template <int D>
 struct PtCfg {
@@ -544,7 +543,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       if (MOD || edge) tc_wait_st();
       TcLd<32>::ld(ts, v[0]);
       const float scale = MOD ? 1.0f : p.scale_log2;
-      const float top = fmaxf(mx[0], mx[1]) * scale - PT_SHIFT;
+      const float top = fmaxf(mx[0], mx[1]) * scale;
       const bool move = top > m + PT_LAZY;
       if (__any_sync(0xffffffffu, move)) {
         const float mn = move ? top : m, a = move ? ex2(m - mn) : 1.0f;
@@ -565,6 +564,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       const float ms = m == -INFINITY ? 0.0f : m;
       // Pass 2: weights, two at a time.
       const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
+      constexpr float W = Half2Of<T>::WEIGHT;
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -578,6 +578,7 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
           a = ex2(a);
           b = ex2(b);
           sum[i & 1] = add2(sum[i & 1], pack2(a, b));
+          if constexpr (W != 1.0f) unpack2(mul2(pack2(a, b), pack2(W, W)), a, b);
           pk[i] = Half2Of<T>::pack(a, b);
         }
         tc_st16(ts + 16 * c, pk);
@@ -602,7 +603,8 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
     }
     const bool whole = pc.begins && pc.ends;
     const int slot = 2 * blockIdx.x + (pc.begins ? 1 : 0);
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    constexpr float W = Half2Of<T>::WEIGHT;
+    const float inv = (l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l)) * (1.0f / W);
     const int64_t row = (int64_t)(r.first + token) * p.Hq + head;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -628,7 +630,12 @@ __device__ __forceinline__ void pt_softmax(const PagedParams& p, uint32_t base, 
       } else {
         uint4* dst = reinterpret_cast<uint4*>(p.ws_o + ((int64_t)slot * PT_ROWS + w * 128 + tid) * D + 32 * c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (W != 1.0f)
+#pragma unroll
+            for (int e = 4 * i; e < 4 * i + 4; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * (1.0f / W));
+          dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
       }
     }
     if (live) {

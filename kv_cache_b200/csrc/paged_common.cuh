@@ -440,10 +440,14 @@ __device__ __forceinline__ uint32_t paged_seen(int t, int lo, int hi) {
   return upto & ~below;
 }
 
+// WEIGHT: what the weights of the second product are multiplied by before they are rounded. A fresh weight is at most 1, a
+// stale one 2^8; times 2^7 they reach 2^15, inside fp16's range, and small ones keep its normal bits down to 2^-21. bf16
+// needs none. The sum of weights is taken without it (a row with one key then has the sum 1 and an exact logarithm).
 template <typename T>
 struct Half2Of;
 template <>
 struct Half2Of<__nv_bfloat16> {
+  static constexpr float WEIGHT = 1.0f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -457,6 +461,7 @@ struct Half2Of<__nv_bfloat16> {
 };
 template <>
 struct Half2Of<__half> {
+  static constexpr float WEIGHT = 128.0f;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
