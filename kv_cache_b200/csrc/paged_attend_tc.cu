@@ -669,7 +669,7 @@ __device__ __forceinline__ void pt_own(PagedPlace& at, PagedRequest& r, long lon
 // sum is taken before that. Rows of K and V that no token of the request sees are zero-filled, not read.
 //
 // 384 threads so that a block's 65536 registers give 208 to a softmax thread and 88 to the others: with
-// 512 threads spills in the issuing warp cost a quarter of the time. Measured, bf16: 2048 tokens on 30720 cached, 32/8 heads
+// 512 threads spills in the issuing warp cost a quarter of the time. Measured, bf16: the last 2048 of 32768 tokens, 32/8 heads
 // (1.07 TFLOP) 0.94-0.98 ms = 1090-1138 TFLOP/s, 0.66-0.69 of the cuBLAS burst rate (1.07 ms under the power cap): 3650
 // cycles per pair of row tiles and key tile, of which the products fill 2048 and the 32768 exponentials, 16 a cycle, 2048.
 template <typename T, int D, bool MOD>
